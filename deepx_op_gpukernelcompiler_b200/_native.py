@@ -34,6 +34,7 @@ ERROR_NAMES = {
 DX_DTYPE_F32 = 0
 DX_DTYPE_F16 = 1
 DX_DTYPE_BF16 = 2
+DX_DTYPE_I8 = 3
 
 DX_ACT_NONE = 0
 DX_ACT_RELU = 1
@@ -79,6 +80,12 @@ SIGNATURES = {
                                              ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
     "dx_fused_gated_linear_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, ctypes.c_int,
                                                                ctypes.c_int]),
+    "dx_quantize_rows": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int, _vp]),
+    "dx_int8_linear": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp]
+                       + [_i64] * 7 + [ctypes.c_int] * 3 + [_vp, ctypes.c_size_t, _vp]),
+    "dx_int8_gated_linear": (ctypes.c_int, [_vp, ctypes.c_int] + [_vp] * 8 + [_i64] * 7
+                             + [ctypes.c_int] * 3 + [_vp, ctypes.c_size_t, _vp]),
+    "dx_int8_workspace_size": (ctypes.c_size_t, [_i64, _i64]),
     "dx_select_kernel": (ctypes.c_int, [_i64, _i64, _i64, ctypes.c_int]),
     "dx_copy_2d_async": (ctypes.c_int, [_vp, ctypes.c_size_t, _vp, ctypes.c_size_t,
                                         ctypes.c_size_t, ctypes.c_size_t, _vp]),

@@ -1524,3 +1524,5 @@ extern "C" int dx_fused_linear_decode_noalloc(const void* X, const void* W, cons
   if (d.mn == 32) return launch_decode<32, __nv_bfloat16>(p, dev, sms, d);
   return launch_decode<64, __nv_bfloat16>(p, dev, sms, d);
 }
+
+#include "dx_int8_api.cuh"

@@ -1,0 +1,635 @@
+// dx_int8.cuh — linear layers on 8-bit integer operands:
+//   Y[m,n] = act(s_m t_n sum_k Xq[m,k] Wq[n,k] + bias[n]) (+ R[m,n])
+//   Y[m,n] = act(s_m tg_n sum_k Xq Wgq + bg[n]) * (s_m tu_n sum_k Xq Wuq + bu[n])
+// with Xq, Wq signed 8-bit, s (one per row of X: token) and t (one per output
+// channel) fp32, fp16 / bf16 / fp32 out.  The sums are exact: 32-bit integer
+// accumulators of tcgen05.mma kind::i8 (K <= 131072, so |sum| < 2^31 even where
+// every product is 128 * 128); they become fp32 once, at the end.
+//
+// Both operands are K-major: rows of 128 bytes of K in 128-byte-swizzled
+// shared memory, one MMA per 32 bytes.  Two kernels:
+//
+//   int8_pair_kernel  CTA pairs, 256 x BN tiles, persistent: the integer form
+//     of umma2_fused_linear_kernel (same roles, barriers and raster).  Serves
+//     problems with enough tiles to fill the GPU.
+//   int8_tile_kernel  one 128 (channels) x MN (tokens) tile per CTA with the
+//     operands swapped — D^T[n, m] — so that a few tokens cost a narrow MMA
+//     while W streams past once; K split over a cluster of C CTAs that add
+//     their integer partial sums through distributed shared memory.  Integer
+//     sums do not depend on their order.  Serves decode, tall-skinny and
+//     ragged problems (its stores have no alignment rule).
+//
+// Every mbarrier wait is bounded, as in dx_umma_gemm.cuh.
+#pragma once
+
+#include "dx_epilogue.cuh"
+#include "dx_ptx.cuh"
+#include "dx_umma_gemm.cuh"
+
+namespace dx {
+
+struct Int8Params {
+  int M, N;
+  int k_blocks;  // 128-byte blocks of K
+  long long ldy, ldr;
+  const float* sx;   // [M]
+  const float* sw;   // [N]
+  const float* sw2;  // gated: the up-projection's [N]
+  const void* bias;
+  const void* bias2;
+  const void* residual;
+  void* Y;
+  int act;
+  // tile kernel
+  int cluster;  // CTAs that split K
+  int w_early;  // the preceding launch wrote only X: W may be read before it ends
+  // pair kernel
+  int m_tiles, num_tiles, n_tiles, group_m, workers;
+  int has_residual;
+};
+
+__device__ __forceinline__ float ld_elem(const void* p, long long i, const __half*) {
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ float ld_elem(const void* p, long long i, const __nv_bfloat16*) {
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ float ld_elem(const void* p, long long i, const float*) {
+  return static_cast<const float*>(p)[i];
+}
+
+// =====================================================================
+// Tile kernel: 128 rows of W x MN tokens, operands swapped.
+// =====================================================================
+template <int MN>
+struct Int8TileShape {
+  static constexpr int BK = 128;             // bytes of K a stage
+  static constexpr int W_BYTES = 128 * BK;   // gated: 64 rows of Wg, 64 of Wu
+  static constexpr int X_BYTES = MN * BK;
+  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
+  // Two CTAs share an SM (113 KB each), so one streams while the other starts
+  // or finishes: as many stages as that leaves.
+  static constexpr int STAGES = MN == 16 ? 6 : (MN == 32 ? 5 : (MN == 64 ? 4 : 3));
+  static constexpr int TMEM_COLS = MN < 32 ? 32 : MN;
+  static constexpr int THREADS = 192;
+  static constexpr int OFF_W = 0;
+  static constexpr int OFF_X = OFF_W + STAGES * W_BYTES;
+  static constexpr int OFF_SX = OFF_X + STAGES * X_BYTES;  // MN row scales
+  static constexpr int OFF_BAR = OFF_SX + MN * 4;
+  static constexpr int BAR_FULL = 0;
+  static constexpr int BAR_EMPTY = STAGES;
+  static constexpr int BAR_TFULL = 2 * STAGES;
+  static constexpr int NUM_BARS = BAR_TFULL + 1;
+  static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
+  static constexpr int SMEM_BYTES = 1024 + OFF_MISC + 16;
+  static constexpr int MAX_CLUSTER = 8;
+  // The partial sums received from a cluster of C CTAs, [source][row of this
+  // CTA's share][128], lie in the idle stage ring: C * ceil(MN / C) rows.
+  static_assert((MN + MAX_CLUSTER) * 128 * 4 <= STAGES * STAGE_BYTES, "receive area");
+  static_assert(SMEM_BYTES <= 115712, "two CTAs per SM");
+};
+
+// First row (of `rows`) of the share that CTA c of C finishes.
+__device__ __forceinline__ int int8_share(int c, int rows, int C) { return c * rows / C; }
+
+template <int MN, typename T, bool kGated>
+__global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
+    int8_tile_kernel(const __grid_constant__ CUtensorMap tmW,
+                     const __grid_constant__ CUtensorMap tmW2,
+                     const __grid_constant__ CUtensorMap tmX, const Int8Params p) {
+  using S = Int8TileShape<MN>;
+  using Tr = ElemTraits<T>;
+  constexpr int NT = kGated ? 64 : 128;  // output channels of the tile
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw_u32 = smem_u32(smem_raw);
+  const uint32_t base = (raw_u32 + 1023u) & ~1023u;
+  uint8_t* const base_ptr = smem_raw + (base - raw_u32);
+  const uint32_t sW = base + S::OFF_W;
+  const uint32_t sX = base + S::OFF_X;
+  const uint32_t bars = base + S::OFF_BAR;
+  float* const s_sx = reinterpret_cast<float*>(base_ptr + S::OFF_SX);
+  uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(base_ptr + S::OFF_MISC);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(base_ptr + S::OFF_MISC + 4);
+  auto bar = [bars](int i) { return bars + 8u * static_cast<uint32_t>(i); };
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int C = p.cluster;
+  const int c = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int n0 = static_cast<int>(blockIdx.x) / C * NT;
+  const int m0 = static_cast<int>(blockIdx.y) * MN;
+  const int rows = min(MN, p.M - m0);
+  const int kb0 = static_cast<int>(static_cast<long long>(c) * p.k_blocks / C);
+  const int kb1 = static_cast<int>(static_cast<long long>(c + 1) * p.k_blocks / C);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(bar(S::BAR_FULL + s), 1);
+      mbar_init(bar(S::BAR_EMPTY + s), 1);
+    }
+    mbar_init(bar(S::BAR_TFULL), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    if (kGated) tma_prefetch_desc(&tmW2);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_word), S::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_word;
+
+  auto load_w = [&](int s, int kb, uint32_t fb, uint64_t pol) {
+    if constexpr (kGated) {
+      tma_load_2d_hint(&tmW, sW + s * S::W_BYTES, fb, kb * S::BK, n0, pol);
+      tma_load_2d_hint(&tmW2, sW + s * S::W_BYTES + S::W_BYTES / 2, fb, kb * S::BK, n0, pol);
+    } else {
+      tma_load_2d_hint(&tmW, sW + s * S::W_BYTES, fb, kb * S::BK, n0, pol);
+    }
+  };
+  const bool producer = warp == 0 && lane == 0;
+  // With one tile of tokens W is read once and leaves L2 first.
+  const uint64_t pol_w =
+      gridDim.y == 1 ? make_l2_policy_evict_first() : make_l2_policy_evict_normal();
+  const int early = min(S::STAGES, kb1 - kb0);
+  if (producer && p.w_early) {
+    for (int i = 0; i < early; ++i) {
+      mbar_arrive_expect_tx(bar(S::BAR_FULL + i), S::STAGE_BYTES);
+      load_w(i, kb0 + i, bar(S::BAR_FULL + i), pol_w);
+    }
+  }
+  __syncwarp();
+  // Everything else in global memory may be the preceding launch's output.
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  const int q = warp & 3;            // TMEM lane quarter of an epilogue warp
+  const int et = threadIdx.x - 64;   // epilogue thread
+  const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  bool done = true;  // epilogue: the accumulator is complete
+  // The channel this epilogue thread finishes, and its scales and biases.
+  const bool via_smem = kGated || C > 1;
+  const int ncol = n0 + (kGated ? (et & 63) : (via_smem ? et : q * 32 + lane));
+  float t0 = 0.0f, t1 = 0.0f, b0 = 0.0f, b1 = 0.0f;
+
+  if (warp == 0) {
+    // ------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t ph = 0;
+      int s = 0, i = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++i) {
+        const uint32_t fb = bar(S::BAR_FULL + s);
+        if (!(p.w_early && i < early)) {
+          if (!mbar_wait(bar(S::BAR_EMPTY + s), ph ^ 1u, abort_flag)) break;
+          mbar_arrive_expect_tx(fb, S::STAGE_BYTES);
+          load_w(s, kb, fb, pol_w);
+        }
+        tma_load_2d(&tmX, sX + s * S::X_BYTES, fb, kb * S::BK, m0);
+        if (++s == S::STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      // Loads in flight land before the shared memory is used or released.
+      const int n_drain = min(i, S::STAGES);
+      for (int j = i - n_drain; j < i; ++j)
+        mbar_wait_drain(bar(S::BAR_FULL + j % S::STAGES), (j / S::STAGES) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_i8(128, MN);
+      uint32_t ph = 0;
+      int s = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(bar(S::BAR_FULL + s), ph, abort_flag)) break;
+        tc_fence_after();
+        const uint64_t ad = smem_desc_sw128(sW + s * S::W_BYTES, 16, 1024);
+        const uint64_t bd = smem_desc_sw128(sX + s * S::X_BYTES, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < S::BK / 32; ++k)
+          umma_i8(tmem, ad + 2ull * k, bd + 2ull * k, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+        umma_commit(bar(S::BAR_EMPTY + s));
+        if (++s == S::STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      umma_commit(bar(S::BAR_TFULL));  // also after a wait that gave up: frees TMEM safely
+      mbar_wait_drain(bar(S::BAR_TFULL), 0);
+    }
+    __syncwarp();
+  } else {
+    // --------------------------------------------------------- epilogue
+    for (int m = et; m < rows; m += 128) s_sx[m] = p.sx[m0 + m];
+    if (ncol < p.N) {
+      t0 = p.sw[ncol];
+      if (p.bias != nullptr) b0 = ld_elem(p.bias, ncol, static_cast<const T*>(nullptr));
+      if (kGated) {
+        t1 = p.sw2[ncol];
+        if (p.bias2 != nullptr) b1 = ld_elem(p.bias2, ncol, static_cast<const T*>(nullptr));
+      }
+    }
+    done = mbar_wait(bar(S::BAR_TFULL), 0, abort_flag) && *abort_flag == 0;
+    tc_fence_after();
+    named_bar_sync(1, 128);  // s_sx
+  }
+
+  T* const Y = static_cast<T*>(p.Y);
+  if (via_smem) {
+    // Partial sums to the CTA that finishes the row, once every ring is idle.
+    if (C > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+    if (warp >= 2 && done) {
+      int dest = 0, end = int8_share(1, rows, C), first = 0;
+#pragma unroll 1
+      for (int mc = 0; mc < rows; mc += 16) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(lane_addr + static_cast<uint32_t>(mc), r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int m = mc + j;
+          if (m < rows) {
+            while (m >= end) {  // at most C steps in all
+              ++dest;
+              first = end;
+              end = int8_share(dest + 1, rows, C);
+            }
+            const uint32_t off =
+                static_cast<uint32_t>(((c * (end - first) + m - first) * 128 + q * 32 + lane) * 4);
+            st_shared_cluster_u32(mapa_shared(base + off, static_cast<uint32_t>(dest)), r[j]);
+          }
+        }
+      }
+    }
+    tc_fence_before();
+    if (C > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+    if (warp >= 2 && done && ncol < p.N) {
+      const int* const recv = reinterpret_cast<const int*>(base_ptr);
+      const int r0 = int8_share(c, rows, C), nr = int8_share(c + 1, rows, C) - r0;
+      constexpr int kStep = kGated ? 2 : 1;
+      for (int i = kGated ? et >> 6 : 0; i < nr; i += kStep) {
+        const long long m = m0 + r0 + i;
+        int a0 = 0, a1 = 0;
+#pragma unroll
+        for (int s = 0; s < S::MAX_CLUSTER; ++s) {
+          if (s < C) {
+            const int* const src = recv + (s * nr + i) * 128 + (kGated ? (et & 63) : et);
+            a0 += src[0];
+            if (kGated) a1 += src[64];
+          }
+        }
+        const float sx = s_sx[r0 + i];
+        float v[1] = {fmaf(static_cast<float>(a0), sx * t0, b0)};
+        act_values(v, p.act);
+        if (kGated) v[0] *= fmaf(static_cast<float>(a1), sx * t1, b1);
+        if (p.residual != nullptr)
+          v[0] += ld_elem(p.residual, m * p.ldr + ncol, static_cast<const T*>(nullptr));
+        Y[m * p.ldy + ncol] = Tr::from_float(v[0]);
+      }
+    }
+  } else if (warp >= 2 && done) {
+#pragma unroll 1
+    for (int mc = 0; mc < rows; mc += 16) {
+      uint32_t r[16];
+      tmem_ld_32x32b_x16(lane_addr + static_cast<uint32_t>(mc), r);
+      float res[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        res[j] = (p.residual != nullptr && ncol < p.N && mc + j < rows)
+                     ? ld_elem(p.residual, (m0 + mc + j) * p.ldr + ncol, static_cast<const T*>(nullptr))
+                     : 0.0f;
+      tmem_wait_ld();
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float sx = mc + j < rows ? s_sx[mc + j] : 0.0f;
+        v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])), sx * t0, b0);
+      }
+      act_values(v, p.act);
+      if (ncol < p.N) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (mc + j < rows) Y[(m0 + mc + j) * p.ldy + ncol] = Tr::from_float(v[j] + res[j]);
+      }
+    }
+    tc_fence_before();
+  }
+
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::TMEM_COLS);
+  }
+}
+
+// =====================================================================
+// CTA-pair kernel: 256 x BN tiles.
+// =====================================================================
+template <int BN>
+struct Int8PairShape {
+  static constexpr int BM = 128;  // rows per CTA
+  static constexpr int BK = 128;
+  static constexpr int BN_CTA = BN / 2;
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int B_BYTES = BN_CTA * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA
+  static constexpr int STAGES = BN == 256 ? 5 : 7;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int THREADS = 64 + 32 * kEpiWarps;
+  static constexpr int VEC_BYTES = 4 * 128 * 4;  // a warp's column scales and biases
+  static constexpr int OFF_A = 0;
+  static constexpr int OFF_B = OFF_A + STAGES * A_BYTES;
+  static constexpr int OFF_EPI = OFF_B + STAGES * B_BYTES;
+  static constexpr int OFF_VEC = OFF_EPI + kEpiWarps * kEpiBufs * kEpiBufBytes;
+  static constexpr int OFF_BAR = OFF_VEC + kEpiWarps * VEC_BYTES;
+  static constexpr int BAR_FULL = 0;
+  static constexpr int BAR_EMPTY = STAGES;
+  static constexpr int BAR_TFULL = 2 * STAGES;
+  static constexpr int BAR_TEMPTY = 2 * STAGES + 2;
+  static constexpr int BAR_RES = 2 * STAGES + 4;
+  static constexpr int BAR_DRAIN = BAR_RES + kEpiBufs * kEpiWarps;
+  static constexpr int NUM_BARS = BAR_DRAIN + 1;
+  static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
+  static constexpr int SMEM_BYTES = 1024 + OFF_MISC + 16;
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+};
+
+// The tile'th tile: m-tiles fastest inside groups of group_m (as umma_tile_coords).
+__device__ __forceinline__ void int8_tile_coords(const Int8Params& p, int t, int& mb, int& nb) {
+  const int per_group = p.group_m * p.n_tiles;
+  const int g = t / per_group;
+  const int r = t - g * per_group;
+  const int m_first = g * p.group_m;
+  const int gm = min(p.group_m, p.m_tiles - m_first);
+  mb = m_first + r % gm;
+  nb = r / gm;
+}
+
+// `cols` column values from n (zeros past N) to a warp's shared array.
+template <typename E>
+__device__ __forceinline__ void int8_stage_vec(float* dst, const E* src, int n, int cols, int N,
+                                               int lane) {
+  for (int j = lane; j < cols; j += 32)
+    dst[j] = (src != nullptr && n + j < N) ? ElemTraits<E>::to_float(src[n + j]) : 0.0f;
+}
+
+// v = acc * (sx * t) + b over the 32 columns at t, b (shared memory, read as
+// broadcasts of four).
+__device__ __forceinline__ void int8_scale(float (&v)[32], const uint32_t (&r)[32], float sx,
+                                           const float* t, const float* b) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 tt = *reinterpret_cast<const float4*>(t + 4 * j);
+    const float4 bb = *reinterpret_cast<const float4*>(b + 4 * j);
+    v[4 * j + 0] = fmaf(static_cast<float>(static_cast<int>(r[4 * j + 0])), sx * tt.x, bb.x);
+    v[4 * j + 1] = fmaf(static_cast<float>(static_cast<int>(r[4 * j + 1])), sx * tt.y, bb.y);
+    v[4 * j + 2] = fmaf(static_cast<float>(static_cast<int>(r[4 * j + 2])), sx * tt.z, bb.z);
+    v[4 * j + 3] = fmaf(static_cast<float>(static_cast<int>(r[4 * j + 3])), sx * tt.w, bb.w);
+  }
+}
+
+template <int BN, typename T, bool kGated>
+__global__ void __launch_bounds__(Int8PairShape<BN>::THREADS, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
+                     const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmB2,
+                     const __grid_constant__ CUtensorMap tmY,
+                     const __grid_constant__ CUtensorMap tmR, const Int8Params p) {
+  using S = Int8PairShape<BN>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw_u32 = smem_u32(smem_raw);
+  const uint32_t base = (raw_u32 + 1023u) & ~1023u;
+  uint8_t* const base_ptr = smem_raw + (base - raw_u32);
+  const uint32_t sA = base + S::OFF_A;
+  const uint32_t sB = base + S::OFF_B;
+  const uint32_t bars = base + S::OFF_BAR;
+  uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(base_ptr + S::OFF_MISC);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(base_ptr + S::OFF_MISC + 4);
+  auto bar = [bars](int i) { return bars + 8u * static_cast<uint32_t>(i); };
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = static_cast<int>(blockIdx.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(bar(S::BAR_FULL + s), 1);
+      mbar_init(bar(S::BAR_EMPTY + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(S::BAR_TFULL + b), 1);
+      mbar_init(bar(S::BAR_TEMPTY + b), 2 * kEpiWarps);
+    }
+    for (int i = 0; i < kEpiBufs * kEpiWarps; ++i) mbar_init(bar(S::BAR_RES + i), 1);
+    mbar_init(bar(S::BAR_DRAIN), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (kGated) tma_prefetch_desc(&tmB2);
+    tma_prefetch_desc(&tmY);
+    if (p.has_residual) tma_prefetch_desc(&tmR);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_word), S::TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_word;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  if (warp == 0) {
+    // ------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const uint64_t pol = make_l2_policy_evict_normal();
+      int s = 0;
+      uint32_t ph = 0, issued = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < p.num_tiles; tile += p.workers) {
+        int mb, nb;
+        int8_tile_coords(p, tile, mb, nb);
+        const int m0 = mb * 2 * S::BM + static_cast<int>(rank) * S::BM;
+        const int n0 = kGated ? nb * S::BN_CTA : nb * BN + static_cast<int>(rank) * S::BN_CTA;
+        const CUtensorMap* const mapB = (kGated && rank != 0) ? &tmB2 : &tmB;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(bar(S::BAR_EMPTY + s), ph ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(bar(S::BAR_FULL + s), 2 * S::STAGE_BYTES);
+          const uint32_t fb = mapa_shared(bar(S::BAR_FULL + s), 0);
+          tma_load_2d_pair(&tmA, sA + s * S::A_BYTES, fb, kb * S::BK, m0, pol);
+          tma_load_2d_pair(mapB, sB + s * S::B_BYTES, fb, kb * S::BK, n0, pol);
+          ++issued;
+          if (++s == S::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (leader) {
+        const uint32_t n_drain = issued < (uint32_t)S::STAGES ? issued : (uint32_t)S::STAGES;
+        for (uint32_t i = issued - n_drain; i < issued; ++i)
+          mbar_wait_drain(bar(S::BAR_FULL + (int)(i % S::STAGES)), (i / S::STAGES) & 1u);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ----------------------------------------------- MMA issuer (leader)
+    if (leader && lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_i8(256, BN);
+      int s = 0, local = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < p.num_tiles; tile += p.workers, ++local) {
+        const int b = local & 1;
+        const uint32_t use_ph = (static_cast<uint32_t>(local) >> 1) & 1u;
+        if (!mbar_wait(bar(S::BAR_TEMPTY + b), use_ph ^ 1u, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * BN);
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(bar(S::BAR_FULL + s), ph, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t ad = smem_desc_sw128(sA + s * S::A_BYTES, 16, 1024);
+          const uint64_t bd = smem_desc_sw128(sB + s * S::B_BYTES, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < S::BK / 32; ++k)
+            umma_i8_pair(d_tmem, ad + 2ull * k, bd + 2ull * k, idesc,
+                         (kb != 0 || k != 0) ? 1u : 0u);
+          umma_commit_pair(mapa_shared(bar(S::BAR_EMPTY + s), 0));
+          umma_commit_pair(mapa_shared(bar(S::BAR_EMPTY + s), 1));
+          if (++s == S::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) {
+          umma_commit_pair(mapa_shared(bar(S::BAR_TFULL + b), 0));
+          umma_commit_pair(mapa_shared(bar(S::BAR_TFULL + b), 1));
+        }
+      }
+      umma_commit_pair(mapa_shared(bar(S::BAR_DRAIN), 0));
+      mbar_wait_drain(bar(S::BAR_DRAIN), 0);
+    }
+    __syncwarp();
+  } else {
+    // --------------------------------------------- epilogue (both CTAs)
+    constexpr int kOut = kGated ? BN / 2 : BN;          // output columns of a tile
+    constexpr int kCols = kOut / kEpiHalves;            // of which this warp's
+    constexpr int kChunks = kCols / 32;
+    const int e = warp - 2;
+    const int q = warp & 3;
+    const int c0 = (e / 4) * kCols;
+    EpilogueCtx<T> c;
+    c.tmY = &tmY;
+    c.tmR = &tmR;
+    c.bias = nullptr;
+    c.M = p.M;
+    c.N = p.N;
+    c.has_residual = p.has_residual;
+    c.ebuf0 = base + S::OFF_EPI + e * kEpiBufs * kEpiBufBytes;
+    c.ebuf_ptr0 = base_ptr + S::OFF_EPI + e * kEpiBufs * kEpiBufBytes;
+    c.rbar0 = bar(S::BAR_RES + e * kEpiBufs);
+    c.pol_stream = make_l2_policy_evict_first();
+    float* const vec = reinterpret_cast<float*>(base_ptr + S::OFF_VEC + e * S::VEC_BYTES);
+    uint32_t it = 0;
+    int local = 0;
+    for (int tile = pair; tile < p.num_tiles; tile += p.workers, ++local) {
+      const int b = local & 1;
+      const uint32_t use_ph = (static_cast<uint32_t>(local) >> 1) & 1u;
+      int mb, nb;
+      int8_tile_coords(p, tile, mb, nb);
+      const int n0 = nb * kOut + c0;
+      const int row_base = mb * 2 * S::BM + static_cast<int>(rank) * S::BM + q * 32;
+      const int row = row_base + lane;
+      const float sx = row < p.M ? p.sx[row] : 0.0f;
+      __syncwarp();  // the previous tile's values are no longer read
+      int8_stage_vec(vec, p.sw, n0, kCols, p.N, lane);
+      int8_stage_vec(vec + 128, static_cast<const T*>(p.bias), n0, kCols, p.N, lane);
+      if (kGated) {
+        int8_stage_vec(vec + 256, p.sw2, n0, kCols, p.N, lane);
+        int8_stage_vec(vec + 384, static_cast<const T*>(p.bias2), n0, kCols, p.N, lane);
+      }
+      __syncwarp();
+      if (!mbar_wait(bar(S::BAR_TFULL + b), use_ph, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t tempty = mapa_shared(bar(S::BAR_TEMPTY + b), 0);
+      const uint32_t acc = tmem_base + static_cast<uint32_t>(b * BN) +
+                           (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(c0);
+      const int live =
+          row_base < p.M && n0 < p.N ? min(kChunks, (p.N - n0 + 31) / 32) : 0;
+      if (live == 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty);
+        continue;
+      }
+      uint32_t r[32], u[32];
+      tmem_ld_32x32b_x32(acc, r);
+      if (kGated) tmem_ld_32x32b_x32(acc + BN / 2, u);
+      bool ok = true;
+#pragma unroll 1
+      for (int ch = 0; ch < live; ++ch) {
+        epi_chunk_begin(c, n0 + 32 * ch, row_base, lane, it);
+        tmem_wait_ld();
+        float v[32], w[32];
+        int8_scale(v, r, sx, vec + 32 * ch, vec + 128 + 32 * ch);
+        if (kGated) int8_scale(w, u, sx, vec + 256 + 32 * ch, vec + 384 + 32 * ch);
+        if (ch + 1 < live) {
+          tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(32 * (ch + 1)), r);
+          if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(BN / 2 + 32 * (ch + 1)), u);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty);
+        }
+        act_values(v, p.act);
+        if (kGated) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= w[j];
+        }
+        if (!epi_chunk_store(c, v, n0 + 32 * ch, row_base, lane, it, abort_flag)) {
+          if (ch + 1 < live) tmem_wait_ld();
+          ok = false;
+          break;
+        }
+      }
+      if (!ok) break;
+    }
+    if (lane == 0) bulk_wait_group<0>();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, S::TMEM_COLS);
+  }
+}
+
+}  // namespace dx

@@ -1,0 +1,415 @@
+// dx_int8_api.cuh — host side of the 8-bit integer linear layers: argument
+// checks, kernel choice, TMA descriptors and launches.  Part of dx_api.cu
+// (it uses that file's helpers).
+#pragma once
+
+#include "dx_int8.cuh"
+#include "dx_quant.cuh"
+
+namespace {
+
+using dx::Int8PairShape;
+using dx::Int8Params;
+using dx::Int8TileShape;
+using dx::QuantParams;
+
+// |sum| <= K * 128 * 128 < 2^31.
+constexpr int64_t kInt8MaxK = 131071;
+
+int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+int elem_size(int dtype) { return dtype == DX_DTYPE_F32 ? 4 : 2; }
+
+bool float_dtype(int dtype) { return dtype >= DX_DTYPE_F32 && dtype <= DX_DTYPE_BF16; }
+
+// 8-bit matrix of `rows` rows of `k` bytes, a [box_rows x 128 byte] box.
+int make_tmap_i8(CUtensorMap* m, const void* ptr, int64_t k, int64_t rows, int64_t ld,
+                 uint32_t box_rows, const char* name) {
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t es[2] = {1, 1};
+  const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims,
+                              strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(DX_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", name,
+                static_cast<int>(r));
+  return DX_OK;
+}
+
+// ---------------------------------------------------------- quantisation
+template <typename T, int THREADS>
+int launch_quantize(const QuantParams& p, cudaStream_t s) {
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = launch_config(p.M, THREADS, 0, s, 1, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, dx::quantize_rows_kernel<T, THREADS>, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "launch quantize_rows_kernel");
+  return DX_OK;
+}
+
+template <typename T>
+int quantize_typed(const QuantParams& p, int sms, cudaStream_t s) {
+  // Few rows: the latency of a row counts, one vector a thread; many: up to
+  // four vectors a thread, all loaded before the first is needed.
+  const int vectors = (p.K + dx::kQuantVec - 1) / dx::kQuantVec;
+  const int threads = p.M <= 4 * sms ? vectors : (vectors + dx::kQuantRegs - 1) / dx::kQuantRegs;
+  if (threads <= 128) return launch_quantize<T, 128>(p, s);
+  if (threads <= 256) return launch_quantize<T, 256>(p, s);
+  if (threads <= 512) return launch_quantize<T, 512>(p, s);
+  return launch_quantize<T, 1024>(p, s);
+}
+
+int run_quantize(const void* X, void* Q, float* scale, int64_t M, int64_t K, int64_t ldx,
+                 int64_t ldq, int dtype, int sms, cudaStream_t s) {
+  QuantParams p{};
+  p.X = X;
+  p.Q = static_cast<int8_t*>(Q);
+  p.scale = scale;
+  p.M = static_cast<int>(M);
+  p.K = static_cast<int>(K);
+  p.ldx = ldx;
+  p.ldq = ldq;
+  p.vec = aligned16(X) && (ldx * elem_size(dtype)) % 16 == 0 && aligned16(Q) && ldq % 8 == 0;
+  if (dtype == DX_DTYPE_F32) return quantize_typed<float>(p, sms, s);
+  if (dtype == DX_DTYPE_F16) return quantize_typed<__half>(p, sms, s);
+  return quantize_typed<__nv_bfloat16>(p, sms, s);
+}
+
+// --------------------------------------------------------------- problem
+struct Int8Problem {
+  const void* X;       // 8-bit rows, or a float type that is quantised first
+  int x_dtype;
+  const float* x_scale;
+  const void *W, *W2;
+  const float *w_scale, *w2_scale;
+  const void *bias, *bias2, *R;
+  void* Y;
+  int64_t M, N, K, ldx, ldw, ldw2, ldr, ldy;
+  int dtype, act, kernel;
+  bool gated;
+  void* ws;
+  size_t ws_bytes;
+  cudaStream_t stream;
+  bool w_early = false;
+};
+
+size_t int8_scale_bytes(int64_t M) { return static_cast<size_t>(round_up(M * 4, 256)); }
+
+size_t int8_workspace(int64_t M, int64_t K) {
+  return int8_scale_bytes(M) + static_cast<size_t>(M) * static_cast<size_t>(round_up(K, 16));
+}
+
+int int8_validate(const Int8Problem& p) {
+  if (!float_dtype(p.dtype)) return fail(DX_ERR_INVALID_ARGUMENT, "unknown dtype %d", p.dtype);
+  if (p.x_dtype != DX_DTYPE_I8 && !float_dtype(p.x_dtype))
+    return fail(DX_ERR_INVALID_ARGUMENT, "unknown x_dtype %d", p.x_dtype);
+  if (p.act < DX_ACT_NONE || p.act > DX_ACT_SILU)
+    return fail(DX_ERR_INVALID_ARGUMENT, "unknown activation %d", p.act);
+  if (p.kernel != DX_KERNEL_AUTO && p.kernel != DX_KERNEL_UMMA && p.kernel != DX_KERNEL_DECODE)
+    return fail(DX_ERR_INVALID_ARGUMENT, "unknown kernel variant %d", p.kernel);
+  if (p.M < 0 || p.N < 0 || p.K < 1)
+    return fail(DX_ERR_INVALID_ARGUMENT, "shape M=%lld N=%lld K=%lld: M, N >= 0 and K >= 1",
+                (long long)p.M, (long long)p.N, (long long)p.K);
+  if (p.K > kInt8MaxK)
+    return fail(DX_ERR_UNSUPPORTED, "K=%lld above %lld, where a 32-bit sum may overflow",
+                (long long)p.K, (long long)kInt8MaxK);
+  if (p.M > (int64_t(1) << 22) || p.N > (int64_t(1) << 24))
+    return fail(DX_ERR_UNSUPPORTED, "M above 2^22 or N above 2^24");
+  if (p.M == 0 || p.N == 0) return DX_OK;
+  if (p.Y == nullptr) return fail(DX_ERR_INVALID_ARGUMENT, "Y is NULL");
+  if (p.X == nullptr || p.W == nullptr || p.w_scale == nullptr ||
+      (p.x_dtype == DX_DTYPE_I8 && p.x_scale == nullptr))
+    return fail(DX_ERR_INVALID_ARGUMENT, "X, W or a scale is NULL");
+  if (p.gated && (p.W2 == nullptr || p.w2_scale == nullptr))
+    return fail(DX_ERR_INVALID_ARGUMENT, "Wu or its scale is NULL");
+  if (p.ldx < p.K)
+    return fail(DX_ERR_INVALID_ARGUMENT, "ldx=%lld < K=%lld", (long long)p.ldx, (long long)p.K);
+  if (p.ldw < p.K || (p.gated && p.ldw2 < p.K))
+    return fail(DX_ERR_INVALID_ARGUMENT, "a weight's pitch is below K=%lld (weights are [N, K])",
+                (long long)p.K);
+  if (p.ldy < p.N)
+    return fail(DX_ERR_INVALID_ARGUMENT, "ldy=%lld < N=%lld", (long long)p.ldy, (long long)p.N);
+  if (p.R != nullptr && p.ldr < p.N)
+    return fail(DX_ERR_INVALID_ARGUMENT, "ldr=%lld < N=%lld", (long long)p.ldr, (long long)p.N);
+  if (!aligned16(p.W) || p.ldw % 16 != 0 || (p.gated && (!aligned16(p.W2) || p.ldw2 % 16 != 0)) ||
+      (p.x_dtype == DX_DTYPE_I8 && (!aligned16(p.X) || p.ldx % 16 != 0)))
+    return fail(DX_ERR_UNSUPPORTED,
+                "8-bit operands need 16-byte-aligned pointers and pitches that are multiples of 16");
+  return DX_OK;
+}
+
+// The pair kernel stores (and reads R) by TMA, in 16-bit types.
+bool int8_pair_eligible(const Int8Problem& p) {
+  return p.dtype != DX_DTYPE_F32 && tma_ok(p.Y, p.ldy) && (p.R == nullptr || tma_ok(p.R, p.ldr));
+}
+
+struct Int8Plan {
+  bool pair = false;
+  int bn = 256;               // pair
+  int workers = 0;            // pair
+  int mn = 16, cluster = 1;   // tile
+};
+
+// Tokens per tile: the fewest that hold M, up to 128.
+int int8_tile_mn(int64_t M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
+
+Int8Plan int8_tile_plan(const Int8Problem& p, int sms) {
+  Int8Plan pl;
+  pl.mn = int8_tile_mn(p.M);
+  const int64_t tiles = ((p.N + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128)) *
+                        ((p.M + pl.mn - 1) / pl.mn);
+  const int64_t k_blocks = (p.K + 127) / 128;
+  // Two CTAs an SM: split K while the CTAs fit, at least two blocks each.
+  for (int c = Int8TileShape<16>::MAX_CLUSTER; c > 1; --c)
+    if (tiles * c <= 2 * sms && k_blocks >= 2 * c) {
+      pl.cluster = c;
+      break;
+    }
+  return pl;
+}
+
+template <int MN, typename T, bool G>
+int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
+  using S = Int8TileShape<MN>;
+  auto kern = dx::int8_tile_kernel<MN, T, G>;
+  int rc = ensure_smem_attr(dev, reinterpret_cast<const void*>(kern), S::SMEM_BYTES, true);
+  if (rc) return rc;
+  constexpr int NT = G ? 64 : 128;
+  CUtensorMap tW, tW2, tX;
+  if ((rc = make_tmap_i8(&tW, pr.W, pr.K, pr.N, pr.ldw, NT, "W"))) return rc;
+  if (G) {
+    if ((rc = make_tmap_i8(&tW2, pr.W2, pr.K, pr.N, pr.ldw2, NT, "W2"))) return rc;
+  } else {
+    tW2 = tW;  // never read
+  }
+  if ((rc = make_tmap_i8(&tX, pr.X, pr.K, pr.M, pr.ldx, MN, "X"))) return rc;
+  Int8Params p{};
+  p.M = static_cast<int>(pr.M);
+  p.N = static_cast<int>(pr.N);
+  p.k_blocks = static_cast<int>((pr.K + 127) / 128);
+  p.ldy = pr.ldy;
+  p.ldr = pr.ldr;
+  p.sx = pr.x_scale;
+  p.sw = pr.w_scale;
+  p.sw2 = pr.w2_scale;
+  p.bias = pr.bias;
+  p.bias2 = pr.bias2;
+  p.residual = pr.R;
+  p.Y = pr.Y;
+  p.act = pr.act;
+  p.cluster = pl.cluster;
+  p.w_early = pr.w_early ? 1 : 0;
+  const int n_tiles = static_cast<int>((pr.N + NT - 1) / NT);
+  const int m_tiles = static_cast<int>((pr.M + MN - 1) / MN);
+  set_plan("int8_tile%s tile=%dx%d stages=%d grid=%dx%d cluster=%d early=%d smem=%d",
+           G ? "_gated" : "", NT, MN, S::STAGES, n_tiles * pl.cluster, m_tiles, pl.cluster,
+           p.w_early, S::SMEM_BYTES);
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = launch_config(n_tiles * pl.cluster, S::THREADS, S::SMEM_BYTES, pr.stream,
+                                         pl.cluster, attr);
+  cfg.gridDim.y = static_cast<unsigned>(m_tiles);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tW, tW2, tX, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "launch int8_tile_kernel");
+  return DX_OK;
+}
+
+template <int BN, typename T, bool G>
+int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
+  using S = Int8PairShape<BN>;
+  auto kern = dx::int8_pair_kernel<BN, T, G>;
+  int rc = ensure_smem_attr(dev, reinterpret_cast<const void*>(kern), S::SMEM_BYTES, false);
+  if (rc) return rc;
+  CUtensorMap tA, tB, tB2, tY, tR;
+  if ((rc = make_tmap_i8(&tA, pr.X, pr.K, pr.M, pr.ldx, 128, "X"))) return rc;
+  if ((rc = make_tmap_i8(&tB, pr.W, pr.K, pr.N, pr.ldw, BN / 2, "W"))) return rc;
+  if (G) {
+    if ((rc = make_tmap_i8(&tB2, pr.W2, pr.K, pr.N, pr.ldw2, BN / 2, "W2"))) return rc;
+  } else {
+    tB2 = tB;  // never read
+  }
+  const CUtensorMapDataType dt = tma_dtype(pr.dtype);
+  if ((rc = make_tmap_2d(&tY, pr.Y, dt, pr.N, pr.M, pr.ldy, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, "Y")))
+    return rc;
+  if (pr.R != nullptr) {
+    if ((rc = make_tmap_2d(&tR, pr.R, dt, pr.N, pr.M, pr.ldr, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B,
+                           "R")))
+      return rc;
+  } else {
+    tR = tY;  // never read
+  }
+  constexpr int NT = G ? BN / 2 : BN;
+  Int8Params p{};
+  p.M = static_cast<int>(pr.M);
+  p.N = static_cast<int>(pr.N);
+  p.k_blocks = static_cast<int>((pr.K + 127) / 128);
+  p.sx = pr.x_scale;
+  p.sw = pr.w_scale;
+  p.sw2 = pr.w2_scale;
+  p.bias = pr.bias;
+  p.bias2 = pr.bias2;
+  p.act = pr.act;
+  p.has_residual = pr.R != nullptr ? 1 : 0;
+  p.m_tiles = static_cast<int>((pr.M + 255) / 256);
+  p.n_tiles = static_cast<int>((pr.N + NT - 1) / NT);
+  p.num_tiles = p.m_tiles * p.n_tiles;
+  p.group_m = pick_group_m(p.m_tiles, 256, (pr.K + 1) / 2);
+  p.workers = std::min(pl.workers, p.num_tiles);
+  set_plan("int8_pair%s tile=256x%d stages=%d grid=%d tiles=%d group_m=%d smem=%d",
+           G ? "_gated" : "", NT, S::STAGES, 2 * p.workers, p.num_tiles, p.group_m, S::SMEM_BYTES);
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg =
+      launch_config(2 * p.workers, S::THREADS, S::SMEM_BYTES, pr.stream, 2, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tA, tB, tB2, tY, tR, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "launch int8_pair_kernel");
+  return DX_OK;
+}
+
+template <typename T, bool G>
+int dispatch_int8_tile(const Int8Problem& p, int dev, const Int8Plan& pl) {
+  switch (pl.mn) {
+    case 16: return launch_int8_tile<16, T, G>(p, dev, pl);
+    case 32: return launch_int8_tile<32, T, G>(p, dev, pl);
+    case 64: return launch_int8_tile<64, T, G>(p, dev, pl);
+    default: return launch_int8_tile<128, T, G>(p, dev, pl);
+  }
+}
+
+template <typename T, bool G>
+int dispatch_int8_pair(const Int8Problem& p, int dev, const Int8Plan& pl) {
+  if constexpr (!G) {
+    if (pl.bn == 128) return launch_int8_pair<128, T, G>(p, dev, pl);
+  }
+  return launch_int8_pair<256, T, G>(p, dev, pl);
+}
+
+template <bool G>
+int dispatch_int8(const Int8Problem& p, int dev, const Int8Plan& pl) {
+  if (pl.pair)
+    return p.dtype == DX_DTYPE_F16 ? dispatch_int8_pair<__half, G>(p, dev, pl)
+                                   : dispatch_int8_pair<__nv_bfloat16, G>(p, dev, pl);
+  if (p.dtype == DX_DTYPE_F32) return dispatch_int8_tile<float, G>(p, dev, pl);
+  return p.dtype == DX_DTYPE_F16 ? dispatch_int8_tile<__half, G>(p, dev, pl)
+                                 : dispatch_int8_tile<__nv_bfloat16, G>(p, dev, pl);
+}
+
+Int8Plan int8_plan(const Int8Problem& p, int dev, int sms) {
+  Int8Plan pl = int8_tile_plan(p, sms);
+  if (p.kernel == DX_KERNEL_DECODE || !int8_pair_eligible(p)) return pl;
+  const int slots = std::min(pair_slots<256, __nv_bfloat16>(dev, sms), sms / 2);
+  if (slots < 1) return pl;
+  const int64_t m_tiles = (p.M + 255) / 256;
+  const int64_t tiles = m_tiles * ((p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256));
+  if (p.kernel == DX_KERNEL_UMMA || (p.M > 128 && tiles >= slots)) {
+    pl.pair = true;
+    pl.workers = slots;
+    const int64_t wide = (tiles + slots - 1) / slots;
+    const int64_t narrow = (m_tiles * ((p.N + 127) / 128) + slots - 1) / slots;
+    pl.bn = !p.gated && narrow < 2 * 0.8 * wide ? 128 : 256;
+  }
+  return pl;
+}
+
+int run_int8(Int8Problem& p) {
+  t_last_error.clear();
+  int rc = int8_validate(p);
+  if (rc) return rc;
+  if (p.M == 0 || p.N == 0) return DX_OK;
+  if (p.kernel == DX_KERNEL_UMMA && !int8_pair_eligible(p))
+    return fail(DX_ERR_UNSUPPORTED,
+                "the CTA-pair kernel needs a 16-bit output and 16-byte-aligned Y and R with row "
+                "pitches that are multiples of 16 bytes");
+  if (p.x_dtype != DX_DTYPE_I8) {
+    const size_t need = int8_workspace(p.M, p.K);
+    if (p.ws == nullptr || p.ws_bytes < need || !aligned16(p.ws))
+      return fail(DX_ERR_WORKSPACE, "a %s X needs a 16-byte-aligned workspace of %zu bytes",
+                  "floating-point", need);
+  }
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  int sms = 0;
+  if ((rc = stream_sms(p.stream, dev, &sms))) return rc;
+  if ((rc = install_status_mirror(dev, p.stream))) return rc;
+  if ((rc = check_status_mirror(dev))) return rc;
+  if (!load_encode_fn())
+    return fail(DX_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  if (p.x_dtype != DX_DTYPE_I8) {
+    float* const scale = static_cast<float*>(p.ws);
+    void* const q = static_cast<char*>(p.ws) + int8_scale_bytes(p.M);
+    const int64_t ldq = round_up(p.K, 16);
+    if ((rc = run_quantize(p.X, q, scale, p.M, p.K, p.ldx, ldq, p.x_dtype, sms, p.stream)))
+      return rc;
+    p.X = q;
+    p.x_scale = scale;
+    p.ldx = ldq;
+    // The launch before the product is the quantisation, which itself waited
+    // for everything before it and writes nothing but q and scale.
+    p.w_early = true;
+  }
+  const Int8Plan pl = int8_plan(p, dev, sms);
+  return p.gated ? dispatch_int8<true>(p, dev, pl) : dispatch_int8<false>(p, dev, pl);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K, int64_t ldx,
+                     int64_t ldq, int dtype, void* stream) {
+  t_last_error.clear();
+  if (!float_dtype(dtype)) return fail(DX_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (M < 0 || K < 0)
+    return fail(DX_ERR_INVALID_ARGUMENT, "negative shape M=%lld K=%lld", (long long)M, (long long)K);
+  if (M > 0x7fffffffLL || K > 0x3fffffffLL)
+    return fail(DX_ERR_UNSUPPORTED, "M above 2^31-1 or K above 2^30-1");
+  if (M == 0) return DX_OK;
+  if (scale == nullptr || (K > 0 && (X == nullptr || Q == nullptr)))
+    return fail(DX_ERR_INVALID_ARGUMENT, "X, Q or scale is NULL");
+  if (ldx < K || ldq < K)
+    return fail(DX_ERR_INVALID_ARGUMENT, "ldx=%lld or ldq=%lld below K=%lld", (long long)ldx,
+                (long long)ldq, (long long)K);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  int sms = 0;
+  int rc = device_sms(dev, &sms);
+  if (rc) return rc;
+  return run_quantize(X, Q, scale, M, K, ldx, ldq, dtype, sms, static_cast<cudaStream_t>(stream));
+}
+
+size_t dx_int8_workspace_size(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || K > kInt8MaxK || M > (int64_t(1) << 22)) return 0;
+  return int8_workspace(M, K);
+}
+
+int dx_int8_linear(const void* X, int x_dtype, const float* x_scale, const void* W,
+                   const float* w_scale, const void* bias, const void* R, void* Y, int64_t M,
+                   int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy,
+                   int dtype, int act, int kernel, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+  Int8Problem p{X,       x_dtype, x_scale, W,   nullptr, w_scale, nullptr, bias, nullptr, R,
+                Y,       M,       N,       K,   ldx,     ldw,     0,       ldr,  ldy,     dtype,
+                act,     kernel,  false,   workspace, workspace_bytes,
+                static_cast<cudaStream_t>(stream)};
+  return run_int8(p);
+}
+
+int dx_int8_gated_linear(const void* X, int x_dtype, const float* x_scale, const void* Wg,
+                         const float* wg_scale, const void* Wu, const float* wu_scale,
+                         const void* bias_g, const void* bias_u, void* Y, int64_t M, int64_t N,
+                         int64_t K, int64_t ldx, int64_t ldwg, int64_t ldwu, int64_t ldy, int dtype,
+                         int act, int kernel, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  Int8Problem p{X,       x_dtype, x_scale, Wg,  Wu,      wg_scale, wu_scale, bias_g, bias_u, nullptr,
+                Y,       M,       N,       K,   ldx,     ldwg,     ldwu,     0,      ldy,    dtype,
+                act,     kernel,  true,    workspace, workspace_bytes,
+                static_cast<cudaStream_t>(stream)};
+  return run_int8(p);
+}
+
+}  // extern "C"

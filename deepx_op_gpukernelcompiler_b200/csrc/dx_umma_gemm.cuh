@@ -206,37 +206,19 @@ __device__ __forceinline__ uint4 epi_load_bias(const EpilogueCtx<T>& c, int n0, 
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+// The rest of a 32-column chunk whose values are final but for the residual:
+// adds it, converts, stages (64-byte swizzle) and TMA-stores.  Returns false if
+// the residual wait gave up.
 template <typename T>
-__device__ __forceinline__ bool epi_chunk_end(const EpilogueCtx<T>& c, float (&v)[32], int n_c,
-                                              int row_base, int lane, uint32_t& it,
-                                              volatile int* abort_flag, uint4 bias_reg, int ch) {
+__device__ __forceinline__ bool epi_chunk_store(const EpilogueCtx<T>& c, float (&v)[32], int n_c,
+                                                int row_base, int lane, uint32_t& it,
+                                                volatile int* abort_flag) {
   using Tr = ElemTraits<T>;
   const int buf = it % kEpiBufs;
   const uint32_t ebuf = c.ebuf0 + buf * kEpiBufBytes;
   uint8_t* const ebp = c.ebuf_ptr0 + buf * kEpiBufBytes;
   const uint32_t row_off = static_cast<uint32_t>(lane) * 64u;
   const uint32_t row_sw = (static_cast<uint32_t>(lane) >> 1) & 3u;  // 64-byte swizzle phase
-  if (c.alpha != 1.0f) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= c.alpha;
-  }
-  if (c.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int src = 4 * ch + j;  // lane holding columns n_c + 8j .. n_c + 8j + 8
-      const uint32_t wv[4] = {__shfl_sync(0xffffffffu, bias_reg.x, src),
-                              __shfl_sync(0xffffffffu, bias_reg.y, src),
-                              __shfl_sync(0xffffffffu, bias_reg.z, src),
-                              __shfl_sync(0xffffffffu, bias_reg.w, src)};
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const float2 f = Tr::unpack2(wv[h]);
-        v[8 * j + 2 * h] += f.x;
-        v[8 * j + 2 * h + 1] += f.y;
-      }
-    }
-  }
-  act_apply_all(v, c.act);
   if (c.has_residual) {
     const uint32_t rbar = c.rbar0 + 8u * buf;
     const uint32_t par = (it / kEpiBufs) & 1u;
@@ -274,6 +256,35 @@ __device__ __forceinline__ bool epi_chunk_end(const EpilogueCtx<T>& c, float (&v
   }
   ++it;
   return true;
+}
+
+template <typename T>
+__device__ __forceinline__ bool epi_chunk_end(const EpilogueCtx<T>& c, float (&v)[32], int n_c,
+                                              int row_base, int lane, uint32_t& it,
+                                              volatile int* abort_flag, uint4 bias_reg, int ch) {
+  using Tr = ElemTraits<T>;
+  if (c.alpha != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= c.alpha;
+  }
+  if (c.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int src = 4 * ch + j;  // lane holding columns n_c + 8j .. n_c + 8j + 8
+      const uint32_t wv[4] = {__shfl_sync(0xffffffffu, bias_reg.x, src),
+                              __shfl_sync(0xffffffffu, bias_reg.y, src),
+                              __shfl_sync(0xffffffffu, bias_reg.z, src),
+                              __shfl_sync(0xffffffffu, bias_reg.w, src)};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const float2 f = Tr::unpack2(wv[h]);
+        v[8 * j + 2 * h] += f.x;
+        v[8 * j + 2 * h + 1] += f.y;
+      }
+    }
+  }
+  act_apply_all(v, c.act);
+  return epi_chunk_store(c, v, n_c, row_base, lane, it, abort_flag);
 }
 
 // Drains this warp's part of one 128 x BN accumulator: TMEM lanes

@@ -1,0 +1,253 @@
+"""8-bit linear layers: the fused linear and the gated dual GEMM on integers.
+
+No reference counterpart; they stand beside ``fused_linear`` and
+``fused_gated_linear`` (linear.py) for models whose weights are kept in 8 bits.
+A matrix of 8-bit rows is an ``Int8Rows`` pair ``(q, scale)``: ``q`` int8 whose
+rows start on 16 bytes, ``scale`` fp32 with one value per row, standing for
+``q * scale[:, None]``.  Activations have a scale per token, weights one per
+output channel and are held as [N, K]: the transpose of the 16-bit layers' W.
+
+    quantize_rows(X)        X [M, K]            -> Int8Rows, one scale per token
+    quantize_weight(W)      W [K, N]            -> Int8Rows [N, K], one per channel
+    int8_rows(q, scale)     8-bit data at hand  -> Int8Rows (rows padded if needed)
+    int8_linear             act(s_m t_n sum_k Xq Wq + bias) + residual
+    int8_gated_linear       act(X Wg^T + bias_g) * (X Wu^T + bias_u)
+    int8_gated_ffn          the gated FFN chain on both
+
+X of a product is an Int8Rows pair or a floating-point matrix, which the call
+quantises first (one launch of its own, whose end overlaps the product's first
+loads of W).  The sums are exact: 32-bit integers, rounded to fp32 once and to
+the output type once.  Inference only: no gradients.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _native as nat
+from .linear import DTYPE_CODES, _check_matrix, _ld, activation_code
+
+# Kernel choices of the 8-bit products: CTA pairs, or one tile per CTA.
+_KERNELS = {"auto": nat.DX_KERNEL_AUTO, "umma": nat.DX_KERNEL_UMMA, "decode": nat.DX_KERNEL_DECODE}
+
+
+class Int8Rows(NamedTuple):
+    """8-bit rows and their scales: the matrix ``q * scale[:, None]``."""
+
+    q: torch.Tensor      # int8 [rows, K], rows starting on 16 bytes
+    scale: torch.Tensor  # float32 [rows]
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        return (self.q.float() * self.scale[:, None]).to(dtype)
+
+
+def _empty_rows(rows: int, K: int, device) -> torch.Tensor:
+    pitch = -(-K // 16) * 16
+    q = torch.empty((rows, pitch), dtype=torch.int8, device=device)
+    return q if pitch == K else q[:, :K]
+
+
+def quantize_rows(X: torch.Tensor) -> Int8Rows:
+    """Each row of X [M, K] as 8-bit integers and a scale.
+
+    With a = max(max |row|, 2^-100): scale = a / 127 and q = 127 x / a rounded
+    to the nearest integer, halves to even, decided exactly.  A row that holds an
+    infinity or a NaN gets the scale NaN, so that products with it are NaN."""
+    if not isinstance(X, torch.Tensor):
+        raise TypeError("X must be a torch tensor")
+    if X.device.type != "cuda":
+        raise ValueError("quantize_rows runs on CUDA tensors only (the engine has no CPU path)")
+    if X.dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {X.dtype}; expected float32, float16 or bfloat16")
+    _check_matrix("X", X, None, None)
+    M, K = X.shape
+    q = _empty_rows(M, K, X.device)
+    scale = torch.empty((M,), dtype=torch.float32, device=X.device)
+    with torch.cuda.device(X.device):
+        rc = nat.load().dx_quantize_rows(
+            X.data_ptr(), q.data_ptr(), scale.data_ptr(), M, K, _ld(X), max(q.stride(0), K),
+            DTYPE_CODES[X.dtype], torch.cuda.current_stream(X.device).cuda_stream)
+    nat.check("dx_quantize_rows", rc)
+    return Int8Rows(q, scale)
+
+
+def quantize_weight(W: torch.Tensor) -> Int8Rows:
+    """W [K, N] of a linear layer as Int8Rows [N, K], one scale per output channel."""
+    _check_matrix("W", W, None, None)
+    return quantize_rows(W.t().contiguous())
+
+
+def int8_rows(q: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
+    """8-bit data at hand as Int8Rows; q is copied only where its rows do not
+    start on 16 bytes."""
+    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise ValueError(f"q must be int8 and scale float32, got {q.dtype} and {scale.dtype}")
+    if q.dim() != 2 or scale.shape != (q.shape[0],):
+        raise ValueError(f"q must be [rows, K] with a scale per row, got {tuple(q.shape)} and "
+                         f"{tuple(scale.shape)}")
+    if (q.stride(1) != 1 or q.data_ptr() % 16
+            or (q.shape[0] > 1 and (q.stride(0) % 16 or q.stride(0) < q.shape[1]))):
+        padded = _empty_rows(q.shape[0], q.shape[1], q.device)
+        padded.copy_(q)
+        q = padded
+    return Int8Rows(q, scale.contiguous())
+
+
+def _pair(name: str, rows, K: int | None, n: int | None) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """Checks an (int8 rows, scales) pair -> (q, scale, pitch)."""
+    if not isinstance(rows, tuple) or len(rows) != 2:
+        raise TypeError(f"{name} must be a pair (int8 rows, float32 scales), see quantize_rows")
+    q, scale = rows
+    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise ValueError(f"{name} must hold int8 rows and float32 scales, got {q.dtype} and "
+                         f"{scale.dtype}")
+    _check_matrix(name, q, n, K)
+    if scale.dim() != 1 or scale.shape[0] != q.shape[0] or not scale.is_contiguous():
+        raise ValueError(f"{name} needs one contiguous scale per row, got {tuple(scale.shape)}")
+    ld = q.stride(0) if q.shape[0] > 1 else -(-q.shape[1] // 16) * 16
+    if ld % 16 or q.data_ptr() % 16:
+        raise ValueError(f"{name}'s rows must start on 16 bytes (pitch {ld}): int8_rows(q, scale) "
+                         f"lays them out")
+    return q, scale, ld
+
+
+def _vector(name: str, b: torch.Tensor | None, N: int) -> None:
+    if b is not None and (b.dim() != 1 or b.shape[0] != N or not b.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous tensor of shape ({N},)")
+
+
+class _Call:
+    """The checks and arguments that both products share."""
+
+    __slots__ = ("name", "x", "x_code", "x_scale", "M", "K", "ldx", "device", "dtype", "act",
+                 "kernel")
+
+    def __init__(self, name, X, dtype, activation, kernel):
+        self.act = activation_code(activation)
+        if kernel not in _KERNELS:
+            raise ValueError(f"unknown kernel {kernel!r}; expected one of {list(_KERNELS)}")
+        self.kernel = _KERNELS[kernel]
+        if isinstance(X, torch.Tensor):
+            if X.dtype not in DTYPE_CODES:
+                raise ValueError(f"unsupported dtype {X.dtype}; expected float32, float16 or "
+                                 f"bfloat16, or a pair (int8 rows, scales)")
+            _check_matrix("X", X, None, None)
+            self.x, self.x_scale, self.ldx = X, None, _ld(X)
+            self.x_code = DTYPE_CODES[X.dtype]
+            self.dtype = X.dtype if dtype is None else dtype
+        else:
+            self.x, self.x_scale, self.ldx = _pair("X", X, None, None)
+            self.x_code = nat.DX_DTYPE_I8
+            self.dtype = torch.bfloat16 if dtype is None else dtype
+        if self.dtype not in DTYPE_CODES:
+            raise ValueError(f"unsupported output dtype {self.dtype}; expected float32, float16 or "
+                             f"bfloat16")
+        self.M, self.K = self.x.shape
+        self.device = self.x.device
+        self.name = name
+        if self.K < 1:
+            raise ValueError("X must have at least one column")
+
+    def check(self, typed, placed) -> None:
+        if self.device.type != "cuda":
+            raise ValueError(f"{self.name} runs on CUDA tensors only (the engine has no CPU path)")
+        for name, t in typed:
+            if t is not None and t.dtype != self.dtype:
+                raise ValueError(f"{name} dtype {t.dtype} differs from the output dtype "
+                                 f"{self.dtype}")
+        for name, t in typed + placed:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, X is on {self.device}")
+
+    def workspace(self) -> torch.Tensor | None:
+        # Of this call alone, from the allocator of the current stream or of the
+        # graph being captured: calls on other streams and other graphs cannot
+        # share it.
+        if self.x_scale is not None or self.M == 0:
+            return None
+        return torch.empty(nat.load().dx_int8_workspace_size(self.M, self.K), dtype=torch.uint8,
+                           device=self.device)
+
+
+def _ptr(t: torch.Tensor | None):
+    return t.data_ptr() if t is not None else None
+
+
+def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
+                residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                dtype: torch.dtype | None = None, kernel: str = "auto") -> torch.Tensor:
+    """Y = act(X Wq^T + bias) + residual on 8-bit operands (dx_int8_linear).
+
+    X: a floating-point matrix [M, K] (quantised here, a scale per token) or an
+    Int8Rows pair.  W: an Int8Rows pair [N, K] (quantize_weight).  Y has X's type,
+    or `dtype` (bfloat16 by default where X is a pair); bias, residual and out
+    have Y's."""
+    c = _Call("int8_linear", X, dtype, activation, kernel)
+    wq, ws, ldw = _pair("W", W, c.K, None)
+    N = wq.shape[0]
+    _vector("bias", bias, N)
+    if residual is not None:
+        _check_matrix("residual", residual, c.M, N)
+    if out is None:
+        out = torch.empty((c.M, N), dtype=c.dtype, device=c.device)
+    else:
+        _check_matrix("out", out, c.M, N)
+    c.check([("bias", bias), ("residual", residual), ("out", out)],
+            [("W", wq), ("W's scale", ws), ("X's scale", c.x_scale)])
+    with torch.cuda.device(c.device):
+        space = c.workspace()
+        rc = nat.load().dx_int8_linear(
+            c.x.data_ptr(), c.x_code, _ptr(c.x_scale), wq.data_ptr(), ws.data_ptr(), _ptr(bias),
+            _ptr(residual), out.data_ptr(), c.M, N, c.K, c.ldx, ldw,
+            _ld(residual) if residual is not None else 0, _ld(out), DTYPE_CODES[c.dtype], c.act,
+            c.kernel, _ptr(space), space.numel() if space is not None else 0,
+            torch.cuda.current_stream(c.device).cuda_stream)
+    nat.check("dx_int8_linear", rc)
+    return out
+
+
+def int8_gated_linear(X, Wg, Wu, bias_g: torch.Tensor | None = None,
+                      bias_u: torch.Tensor | None = None, activation="silu",
+                      out: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+                      kernel: str = "auto") -> torch.Tensor:
+    """Y = act(X Wg^T + bias_g) * (X Wu^T + bias_u) on 8-bit operands, X read
+    once for both weights (dx_int8_gated_linear).  Arguments as int8_linear."""
+    c = _Call("int8_gated_linear", X, dtype, activation, kernel)
+    gq, gs, ldg = _pair("Wg", Wg, c.K, None)
+    N = gq.shape[0]
+    uq, us, ldu = _pair("Wu", Wu, c.K, N)
+    _vector("bias_g", bias_g, N)
+    _vector("bias_u", bias_u, N)
+    if out is None:
+        out = torch.empty((c.M, N), dtype=c.dtype, device=c.device)
+    else:
+        _check_matrix("out", out, c.M, N)
+    c.check([("bias_g", bias_g), ("bias_u", bias_u), ("out", out)],
+            [("Wg", gq), ("Wg's scale", gs), ("Wu", uq), ("Wu's scale", us),
+             ("X's scale", c.x_scale)])
+    with torch.cuda.device(c.device):
+        space = c.workspace()
+        rc = nat.load().dx_int8_gated_linear(
+            c.x.data_ptr(), c.x_code, _ptr(c.x_scale), gq.data_ptr(), gs.data_ptr(), uq.data_ptr(),
+            us.data_ptr(), _ptr(bias_g), _ptr(bias_u), out.data_ptr(), c.M, N, c.K, c.ldx, ldg,
+            ldu, _ld(out), DTYPE_CODES[c.dtype], c.act, c.kernel, _ptr(space),
+            space.numel() if space is not None else 0,
+            torch.cuda.current_stream(c.device).cuda_stream)
+    nat.check("dx_int8_gated_linear", rc)
+    return out
+
+
+def int8_gated_ffn(X, Wg, bg: torch.Tensor | None, Wu, bu: torch.Tensor | None, Wo,
+                   bo: torch.Tensor | None, activation="silu",
+                   residual: torch.Tensor | None = None, hidden: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None,
+                   dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Y = H Wo^T + bo + residual with H = act(X Wg^T + bg) * (X Wu^T + bu), all
+    three weights in 8 bits.  H has Y's type between the two products (`hidden`
+    optionally receives it) and is quantised per token again."""
+    if isinstance(Wg, tuple) and isinstance(Wo, tuple) and Wo[0].shape[1] != Wg[0].shape[0]:
+        raise ValueError(f"Wo must take the hidden width {Wg[0].shape[0]}, got "
+                         f"{tuple(Wo[0].shape)}")
+    H = int8_gated_linear(X, Wg, Wu, bg, bu, activation, out=hidden, dtype=dtype)
+    return int8_linear(H, Wo, bo, None, residual=residual, out=out)

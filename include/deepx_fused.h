@@ -58,6 +58,8 @@ extern "C" {
 #define DX_DTYPE_F32   0   /* exact fp32 FFMA path (no TF32)                 */
 #define DX_DTYPE_F16   1   /* tcgen05 kind::f16, fp32 accumulate             */
 #define DX_DTYPE_BF16  2   /* tcgen05 kind::f16 (bf16), fp32 accumulate      */
+#define DX_DTYPE_I8    3   /* signed 8-bit rows with a scale each (an X of
+                              dx_int8_linear / dx_int8_gated_linear only)    */
 
 /* ---- activations (fusion.py ACTIVATION_PT + the kernels' erf GELU) ------ */
 #define DX_ACT_NONE       0  /* pattern `linear`                             */
@@ -279,6 +281,51 @@ int dx_copy_2d_async(void* dst, size_t dst_pitch, const void* src, size_t src_pi
 /* Workspace bytes that dx_fused_gated_linear needs (0: none). */
 size_t dx_fused_gated_linear_workspace_size(int64_t M, int64_t N, int64_t K,
                                             int dtype, int kernel);
+
+/*
+ * 8-bit linear layers (no reference counterpart): the fused linear and the
+ * gated dual GEMM on signed 8-bit operands with one fp32 scale per row of X
+ * (token) and per row of W (output channel).  Weights are [N, K] — each
+ * channel's K values contiguous, the transpose of the 16-bit layers' W.
+ *
+ * dx_quantize_rows: a = max(max_k |X[m,k]|, 2^-100), scale[m] = a / 127,
+ * Q[m,k] = the integer nearest 127 X[m,k] / a, halves to even.  A row with an
+ * infinity or NaN gets scale NaN and zeros.  Any pitch and alignment; bytes of
+ * Q's rows behind K are left alone.
+ */
+int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K, int64_t ldx,
+                     int64_t ldq, int dtype, void* stream);
+
+/*
+ * Y = act(x_scale[m] w_scale[n] sum_k Xq[m,k] Wq[n,k] + bias[n]) + R[m,n].
+ * X is 8-bit with its scales (x_dtype = DX_DTYPE_I8; 16-byte-aligned, ldx a
+ * multiple of 16) or a floating-point type, which the call quantises first as
+ * dx_quantize_rows does (x_scale unused, and a 16-byte-aligned workspace of
+ * dx_int8_workspace_size() bytes, which no other call may use meanwhile; it
+ * needs no initial value).  bias, R and Y have type `dtype`; W is
+ * 16-byte-aligned with ldw a multiple of 16.  The sums are exact (32-bit
+ * integers, 1 <= K <= 131071) and become fp32 once.  `kernel` is
+ * DX_KERNEL_AUTO, DX_KERNEL_UMMA (CTA pairs; 16-bit outputs whose rows are
+ * 16-byte aligned) or DX_KERNEL_DECODE (one tile per CTA, any output).
+ */
+int dx_int8_linear(const void* X, int x_dtype, const float* x_scale, const void* W,
+                   const float* w_scale, const void* bias, const void* R, void* Y, int64_t M,
+                   int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy,
+                   int dtype, int act, int kernel, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* Y = act(x_scale wg_scale Xq Wgq^T + bias_g) * (x_scale wu_scale Xq Wuq^T + bias_u);
+ * otherwise as dx_int8_linear, without a residual. */
+int dx_int8_gated_linear(const void* X, int x_dtype, const float* x_scale, const void* Wg,
+                         const float* wg_scale, const void* Wu, const float* wu_scale,
+                         const void* bias_g, const void* bias_u, void* Y, int64_t M, int64_t N,
+                         int64_t K, int64_t ldx, int64_t ldwg, int64_t ldwu, int64_t ldy, int dtype,
+                         int act, int kernel, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Workspace bytes dx_int8_linear and dx_int8_gated_linear need for a
+ * floating-point X of M rows of K values. */
+size_t dx_int8_workspace_size(int64_t M, int64_t K);
 
 /*
  * Plans — the compile-then-call runtime of the reference design docs: the
