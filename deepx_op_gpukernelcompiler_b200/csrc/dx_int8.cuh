@@ -9,10 +9,10 @@
 // Both operands are K-major: rows of 128 bytes of K in 128-byte-swizzled
 // shared memory, one MMA per 32 bytes.  Two kernels:
 //
-//   int8_pair_kernel  CTA pairs, 256 x BN tiles, persistent: the integer form
+//   int8_pair_kernel  CTA pairs, 256 x bn tiles, persistent: the integer form
 //     of umma2_fused_linear_kernel (same roles, barriers and raster).  Serves
 //     problems with enough tiles to fill the GPU.
-//   int8_tile_kernel  one 128 (channels) x MN (tokens) tile per CTA with the
+//   int8_tile_kernel  one 128 (channels) x mn (tokens) tile per CTA with the
 //     operands swapped — D^T[n, m] — so that a few tokens cost a narrow MMA
 //     while W streams past once; K split over a cluster of C CTAs that add
 //     their integer partial sums through distributed shared memory.  Integer
@@ -41,9 +41,12 @@ struct Int8Params {
   void* Y;
   int act;
   // tile kernel
+  int mn;       // tokens of a tile: a multiple of 16 up to 128
   int cluster;  // CTAs that split K
   int w_early;  // the preceding launch wrote only X: W may be read before it ends
+  int stages;   // of the operand ring (both kernels)
   // pair kernel
+  int bn;       // accumulator columns of a tile: a multiple of 32 (gated: 64) up to 256
   int m_tiles, num_tiles, n_tiles, group_m, workers;
   int has_residual;
 };
@@ -59,71 +62,77 @@ __device__ __forceinline__ float ld_elem(const void* p, long long i, const float
 }
 
 // =====================================================================
-// Tile kernel: 128 rows of W x MN tokens, operands swapped.
+// Tile kernel: 128 rows of W x mn tokens, operands swapped.
 // =====================================================================
-template <int MN>
 struct Int8TileShape {
-  static constexpr int BK = 128;             // bytes of K a stage
-  static constexpr int W_BYTES = 128 * BK;   // gated: 64 rows of Wg, 64 of Wu
-  static constexpr int X_BYTES = MN * BK;
-  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
-  // Two CTAs share an SM (113 KB each), so one streams while the other starts
-  // or finishes: as many stages as that leaves.
-  static constexpr int STAGES = MN == 16 ? 6 : (MN == 32 ? 5 : (MN == 64 ? 4 : 3));
-  static constexpr int TMEM_COLS = MN < 32 ? 32 : MN;
+  static constexpr int MAX_MN = 128;
+  static constexpr int BK = 128;            // bytes of K a stage
+  static constexpr int W_BYTES = 128 * BK;  // gated: 64 rows of Wg, 64 of Wu
+  static constexpr int MAX_STAGES = 12;
+  static constexpr int MAX_CLUSTER = 8;
   static constexpr int THREADS = 192;
-  static constexpr int OFF_W = 0;
-  static constexpr int OFF_X = OFF_W + STAGES * W_BYTES;
-  static constexpr int OFF_SX = OFF_X + STAGES * X_BYTES;  // MN row scales
-  static constexpr int OFF_BAR = OFF_SX + MN * 4;
+  // Shared memory: the ring of `stages` W tiles, then as many X tiles, then
+  static constexpr int OFF_BAR = MAX_MN * 4;  // (behind MAX_MN row scales)
   static constexpr int BAR_FULL = 0;
-  static constexpr int BAR_EMPTY = STAGES;
-  static constexpr int BAR_TFULL = 2 * STAGES;
+  static constexpr int BAR_EMPTY = MAX_STAGES;
+  static constexpr int BAR_TFULL = 2 * MAX_STAGES;
   static constexpr int NUM_BARS = BAR_TFULL + 1;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  static constexpr int SMEM_BYTES = 1024 + OFF_MISC + 16;
-  static constexpr int MAX_CLUSTER = 8;
+  static constexpr int TAIL_BYTES = OFF_MISC + 16;
+  static constexpr int stage_bytes(int mn) { return W_BYTES + mn * BK; }
+  static constexpr int smem_bytes(int mn, int stages) {
+    return 1024 + stages * stage_bytes(mn) + TAIL_BYTES;
+  }
+  static constexpr int HALF_SM = 115712;  // what each of two CTAs of an SM may have
+  static constexpr int FULL_SM = 227 * 1024;
   // The partial sums received from a cluster of C CTAs, [source][row of this
-  // CTA's share][128], lie in the idle stage ring: C * ceil(MN / C) rows.
-  static_assert((MN + MAX_CLUSTER) * 128 * 4 <= STAGES * STAGE_BYTES, "receive area");
-  static_assert(SMEM_BYTES <= 115712, "two CTAs per SM");
+  // CTA's share][128], lie in the idle ring: at most mn + C rows of 512 bytes.
+  static constexpr bool receive_fits(int mn, int stages) {
+    return (mn + MAX_CLUSTER) * 512 <= stages * stage_bytes(mn);
+  }
 };
 
 // First row (of `rows`) of the share that CTA c of C finishes.
 __device__ __forceinline__ int int8_share(int c, int rows, int C) { return c * rows / C; }
 
-template <int MN, typename T, bool kGated>
-__global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
+template <typename T, bool kGated>
+__global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
     int8_tile_kernel(const __grid_constant__ CUtensorMap tmW,
                      const __grid_constant__ CUtensorMap tmW2,
                      const __grid_constant__ CUtensorMap tmX, const Int8Params p) {
-  using S = Int8TileShape<MN>;
+  using S = Int8TileShape;
   using Tr = ElemTraits<T>;
   constexpr int NT = kGated ? 64 : 128;  // output channels of the tile
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base = (raw_u32 + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw_u32);
-  const uint32_t sW = base + S::OFF_W;
-  const uint32_t sX = base + S::OFF_X;
-  const uint32_t bars = base + S::OFF_BAR;
-  float* const s_sx = reinterpret_cast<float*>(base_ptr + S::OFF_SX);
-  uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(base_ptr + S::OFF_MISC);
-  volatile int* const abort_flag = reinterpret_cast<volatile int*>(base_ptr + S::OFF_MISC + 4);
+  const int stages = p.stages;
+  const uint32_t x_bytes = static_cast<uint32_t>(p.mn) * S::BK;
+  const uint32_t stage_bytes = S::W_BYTES + x_bytes;
+  const uint32_t sW = base;
+  const uint32_t sX = base + static_cast<uint32_t>(stages) * S::W_BYTES;
+  const uint32_t tail = static_cast<uint32_t>(stages) * stage_bytes;
+  const uint32_t bars = base + tail + S::OFF_BAR;
+  float* const s_sx = reinterpret_cast<float*>(base_ptr + tail);
+  uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(base_ptr + tail + S::OFF_MISC);
+  volatile int* const abort_flag =
+      reinterpret_cast<volatile int*>(base_ptr + tail + S::OFF_MISC + 4);
+  const uint32_t tmem_cols = p.mn <= 32 ? 32u : (p.mn <= 64 ? 64u : 128u);
   auto bar = [bars](int i) { return bars + 8u * static_cast<uint32_t>(i); };
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int C = p.cluster;
   const int c = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int n0 = static_cast<int>(blockIdx.x) / C * NT;
-  const int m0 = static_cast<int>(blockIdx.y) * MN;
-  const int rows = min(MN, p.M - m0);
+  const int m0 = static_cast<int>(blockIdx.y) * p.mn;
+  const int rows = min(p.mn, p.M - m0);
   const int kb0 = static_cast<int>(static_cast<long long>(c) * p.k_blocks / C);
   const int kb1 = static_cast<int>(static_cast<long long>(c + 1) * p.k_blocks / C);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(bar(S::BAR_FULL + s), 1);
       mbar_init(bar(S::BAR_EMPTY + s), 1);
     }
@@ -137,7 +146,7 @@ __global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
     tma_prefetch_desc(&tmX);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_word), S::TMEM_COLS);
+    tmem_alloc(smem_u32(tmem_word), tmem_cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -157,10 +166,10 @@ __global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
   // With one tile of tokens W is read once and leaves L2 first.
   const uint64_t pol_w =
       gridDim.y == 1 ? make_l2_policy_evict_first() : make_l2_policy_evict_normal();
-  const int early = min(S::STAGES, kb1 - kb0);
+  const int early = min(stages, kb1 - kb0);
   if (producer && p.w_early) {
     for (int i = 0; i < early; ++i) {
-      mbar_arrive_expect_tx(bar(S::BAR_FULL + i), S::STAGE_BYTES);
+      mbar_arrive_expect_tx(bar(S::BAR_FULL + i), stage_bytes);
       load_w(i, kb0 + i, bar(S::BAR_FULL + i), pol_w);
     }
   }
@@ -187,48 +196,52 @@ __global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
         const uint32_t fb = bar(S::BAR_FULL + s);
         if (!(p.w_early && i < early)) {
           if (!mbar_wait(bar(S::BAR_EMPTY + s), ph ^ 1u, abort_flag)) break;
-          mbar_arrive_expect_tx(fb, S::STAGE_BYTES);
+          mbar_arrive_expect_tx(fb, stage_bytes);
           load_w(s, kb, fb, pol_w);
         }
-        tma_load_2d(&tmX, sX + s * S::X_BYTES, fb, kb * S::BK, m0);
-        if (++s == S::STAGES) {
+        tma_load_2d(&tmX, sX + s * x_bytes, fb, kb * S::BK, m0);
+        if (++s == stages) {
           s = 0;
           ph ^= 1u;
         }
       }
       // Loads in flight land before the shared memory is used or released.
-      const int n_drain = min(i, S::STAGES);
+      const int n_drain = min(i, stages);
       for (int j = i - n_drain; j < i; ++j)
-        mbar_wait_drain(bar(S::BAR_FULL + j % S::STAGES), (j / S::STAGES) & 1);
+        mbar_wait_drain(bar(S::BAR_FULL + j % stages), (j / stages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc_i8(128, MN);
-      uint32_t ph = 0;
-      int s = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(bar(S::BAR_FULL + s), ph, abort_flag)) break;
-        tc_fence_after();
-        const uint64_t ad = smem_desc_sw128(sW + s * S::W_BYTES, 16, 1024);
-        const uint64_t bd = smem_desc_sw128(sX + s * S::X_BYTES, 16, 1024);
+    // The whole warp runs the loop and one lane issues: with every operand the
+    // same in all lanes the descriptors stay in uniform registers.  A loop of
+    // lane 0 alone took 165 ns a stage plus 29 ns an MMA to issue.
+    const uint32_t idesc = umma_idesc_i8(128, p.mn);
+    const bool issuer = elect_one();
+    uint32_t ph = 0;
+    int s = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(bar(S::BAR_FULL + s), ph, abort_flag)) break;
+      const uint64_t ad = smem_desc_sw128(sW + s * S::W_BYTES, 16, 1024);
+      const uint64_t bd = smem_desc_sw128(sX + s * x_bytes, 16, 1024);
+      if (issuer) {
 #pragma unroll
         for (int k = 0; k < S::BK / 32; ++k)
           umma_i8(tmem, ad + 2ull * k, bd + 2ull * k, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
         umma_commit(bar(S::BAR_EMPTY + s));
-        if (++s == S::STAGES) {
-          s = 0;
-          ph ^= 1u;
-        }
       }
-      umma_commit(bar(S::BAR_TFULL));  // also after a wait that gave up: frees TMEM safely
-      mbar_wait_drain(bar(S::BAR_TFULL), 0);
+      __syncwarp();
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
+      }
     }
+    if (issuer) umma_commit(bar(S::BAR_TFULL));  // also after a wait that gave up
+    mbar_wait_drain(bar(S::BAR_TFULL), 0);
     __syncwarp();
   } else {
     // --------------------------------------------------------- epilogue
-    for (int m = et; m < rows; m += 128) s_sx[m] = p.sx[m0 + m];
+    if (et < rows) s_sx[et] = p.sx[m0 + et];
     if (ncol < p.N) {
       t0 = p.sw[ncol];
       if (p.bias != nullptr) b0 = ld_elem(p.bias, ncol, static_cast<const T*>(nullptr));
@@ -294,7 +307,7 @@ __global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
         }
         const float sx = s_sx[r0 + i];
         float v[1] = {fmaf(static_cast<float>(a0), sx * t0, b0)};
-        act_values(v, p.act);
+        act_values<sizeof(T) == 4>(v, p.act);
         if (kGated) v[0] *= fmaf(static_cast<float>(a1), sx * t1, b1);
         if (p.residual != nullptr)
           v[0] += ld_elem(p.residual, m * p.ldr + ncol, static_cast<const T*>(nullptr));
@@ -319,7 +332,7 @@ __global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
         const float sx = mc + j < rows ? s_sx[mc + j] : 0.0f;
         v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])), sx * t0, b0);
       }
-      act_values(v, p.act);
+      act_values<sizeof(T) == 4>(v, p.act);
       if (ncol < p.N) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -332,36 +345,34 @@ __global__ void __launch_bounds__(Int8TileShape<MN>::THREADS, 2)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, S::TMEM_COLS);
+    tmem_dealloc(tmem, tmem_cols);
   }
 }
 
 // =====================================================================
-// CTA-pair kernel: 256 x BN tiles.
+// CTA-pair kernel: 256 x bn tiles, bn chosen for each problem.
 // =====================================================================
-template <int BN>
 struct Int8PairShape {
   static constexpr int BM = 128;  // rows per CTA
   static constexpr int BK = 128;
-  static constexpr int BN_CTA = BN / 2;
+  static constexpr int MAX_BN = 256;
   static constexpr int A_BYTES = BM * BK;
-  static constexpr int B_BYTES = BN_CTA * BK;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA
-  static constexpr int STAGES = BN == 256 ? 5 : 7;
-  static constexpr int TMEM_COLS = 2 * BN;
+  // The ring holds as many stages of A_BYTES + bn / 2 * BK as fit (5 at bn = 256).
+  static constexpr int RING_BYTES = 5 * (A_BYTES + MAX_BN / 2 * BK);
+  static constexpr int MAX_STAGES = 8;
+  static constexpr int TMEM_COLS = 2 * MAX_BN;  // two accumulators
   static constexpr int THREADS = 64 + 32 * kEpiWarps;
   static constexpr int VEC_BYTES = 4 * 128 * 4;  // a warp's column scales and biases
-  static constexpr int OFF_A = 0;
-  static constexpr int OFF_B = OFF_A + STAGES * A_BYTES;
-  static constexpr int OFF_EPI = OFF_B + STAGES * B_BYTES;
-  static constexpr int OFF_VEC = OFF_EPI + kEpiWarps * kEpiBufs * kEpiBufBytes;
+  static constexpr int OFF_EPI = RING_BYTES;
+  static constexpr int EPI_BUFS = 3;  // staging buffers of an epilogue warp
+  static constexpr int OFF_VEC = OFF_EPI + kEpiWarps * EPI_BUFS * kEpiBufBytes;
   static constexpr int OFF_BAR = OFF_VEC + kEpiWarps * VEC_BYTES;
   static constexpr int BAR_FULL = 0;
-  static constexpr int BAR_EMPTY = STAGES;
-  static constexpr int BAR_TFULL = 2 * STAGES;
-  static constexpr int BAR_TEMPTY = 2 * STAGES + 2;
-  static constexpr int BAR_RES = 2 * STAGES + 4;
-  static constexpr int BAR_DRAIN = BAR_RES + kEpiBufs * kEpiWarps;
+  static constexpr int BAR_EMPTY = MAX_STAGES;
+  static constexpr int BAR_TFULL = 2 * MAX_STAGES;
+  static constexpr int BAR_TEMPTY = BAR_TFULL + 2;
+  static constexpr int BAR_RES = BAR_TEMPTY + 2;
+  static constexpr int BAR_DRAIN = BAR_RES + EPI_BUFS * kEpiWarps;
   static constexpr int NUM_BARS = BAR_DRAIN + 1;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int SMEM_BYTES = 1024 + OFF_MISC + 16;
@@ -402,33 +413,35 @@ __device__ __forceinline__ void int8_scale(float (&v)[32], const uint32_t (&r)[3
   }
 }
 
-template <int BN, typename T, bool kGated>
-__global__ void __launch_bounds__(Int8PairShape<BN>::THREADS, 1)
+template <typename T, bool kGated>
+__global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                      const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmB2,
                      const __grid_constant__ CUtensorMap tmY,
                      const __grid_constant__ CUtensorMap tmR, const Int8Params p) {
-  using S = Int8PairShape<BN>;
+  using S = Int8PairShape;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base = (raw_u32 + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw_u32);
-  const uint32_t sA = base + S::OFF_A;
-  const uint32_t sB = base + S::OFF_B;
+  const int bn_cta = p.bn / 2;  // W rows staged by each CTA
+  const uint32_t b_bytes = static_cast<uint32_t>(bn_cta) * S::BK;
+  const uint32_t sA = base;
+  const uint32_t sB = base + static_cast<uint32_t>(p.stages) * S::A_BYTES;
   const uint32_t bars = base + S::OFF_BAR;
   uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(base_ptr + S::OFF_MISC);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(base_ptr + S::OFF_MISC + 4);
   auto bar = [bars](int i) { return bars + 8u * static_cast<uint32_t>(i); };
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int pair = static_cast<int>(blockIdx.x >> 1);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::STAGES; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(bar(S::BAR_FULL + s), 1);
       mbar_init(bar(S::BAR_EMPTY + s), 1);
     }
@@ -436,7 +449,7 @@ __global__ void __launch_bounds__(Int8PairShape<BN>::THREADS, 1)
       mbar_init(bar(S::BAR_TFULL + b), 1);
       mbar_init(bar(S::BAR_TEMPTY + b), 2 * kEpiWarps);
     }
-    for (int i = 0; i < kEpiBufs * kEpiWarps; ++i) mbar_init(bar(S::BAR_RES + i), 1);
+    for (int i = 0; i < S::EPI_BUFS * kEpiWarps; ++i) mbar_init(bar(S::BAR_RES + i), 1);
     mbar_init(bar(S::BAR_DRAIN), 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -470,80 +483,82 @@ __global__ void __launch_bounds__(Int8PairShape<BN>::THREADS, 1)
         int mb, nb;
         int8_tile_coords(p, tile, mb, nb);
         const int m0 = mb * 2 * S::BM + static_cast<int>(rank) * S::BM;
-        const int n0 = kGated ? nb * S::BN_CTA : nb * BN + static_cast<int>(rank) * S::BN_CTA;
+        const int n0 = kGated ? nb * bn_cta : nb * p.bn + static_cast<int>(rank) * bn_cta;
         const CUtensorMap* const mapB = (kGated && rank != 0) ? &tmB2 : &tmB;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!mbar_wait(bar(S::BAR_EMPTY + s), ph ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          if (leader) mbar_arrive_expect_tx(bar(S::BAR_FULL + s), 2 * S::STAGE_BYTES);
+          if (leader) mbar_arrive_expect_tx(bar(S::BAR_FULL + s), 2 * (S::A_BYTES + b_bytes));
           const uint32_t fb = mapa_shared(bar(S::BAR_FULL + s), 0);
           tma_load_2d_pair(&tmA, sA + s * S::A_BYTES, fb, kb * S::BK, m0, pol);
-          tma_load_2d_pair(mapB, sB + s * S::B_BYTES, fb, kb * S::BK, n0, pol);
+          tma_load_2d_pair(mapB, sB + s * b_bytes, fb, kb * S::BK, n0, pol);
           ++issued;
-          if (++s == S::STAGES) {
+          if (++s == p.stages) {
             s = 0;
             ph ^= 1u;
           }
         }
       }
       if (leader) {
-        const uint32_t n_drain = issued < (uint32_t)S::STAGES ? issued : (uint32_t)S::STAGES;
+        const uint32_t stages = static_cast<uint32_t>(p.stages);
+        const uint32_t n_drain = issued < stages ? issued : stages;
         for (uint32_t i = issued - n_drain; i < issued; ++i)
-          mbar_wait_drain(bar(S::BAR_FULL + (int)(i % S::STAGES)), (i / S::STAGES) & 1u);
+          mbar_wait_drain(bar(S::BAR_FULL + static_cast<int>(i % stages)), (i / stages) & 1u);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     // ----------------------------------------------- MMA issuer (leader)
-    if (leader && lane == 0) {
-      constexpr uint32_t idesc = umma_idesc_i8(256, BN);
+    if (leader) {
+      const uint32_t idesc = umma_idesc_i8(256, p.bn);
+      const bool issuer = elect_one();
       int s = 0, local = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < p.num_tiles; tile += p.workers, ++local) {
         const int b = local & 1;
         const uint32_t use_ph = (static_cast<uint32_t>(local) >> 1) & 1u;
-        if (!mbar_wait(bar(S::BAR_TEMPTY + b), use_ph ^ 1u, abort_flag)) break;
+        if (!mbar_wait_warp(bar(S::BAR_TEMPTY + b), use_ph ^ 1u, abort_flag)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * BN);
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * S::MAX_BN);
         for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!mbar_wait(bar(S::BAR_FULL + s), ph, abort_flag)) {
+          if (!mbar_wait_warp(bar(S::BAR_FULL + s), ph, abort_flag)) {
             ok = false;
             break;
           }
-          tc_fence_after();
           const uint64_t ad = smem_desc_sw128(sA + s * S::A_BYTES, 16, 1024);
-          const uint64_t bd = smem_desc_sw128(sB + s * S::B_BYTES, 16, 1024);
+          const uint64_t bd = smem_desc_sw128(sB + s * b_bytes, 16, 1024);
+          if (issuer) {
 #pragma unroll
-          for (int k = 0; k < S::BK / 32; ++k)
-            umma_i8_pair(d_tmem, ad + 2ull * k, bd + 2ull * k, idesc,
-                         (kb != 0 || k != 0) ? 1u : 0u);
-          umma_commit_pair(mapa_shared(bar(S::BAR_EMPTY + s), 0));
-          umma_commit_pair(mapa_shared(bar(S::BAR_EMPTY + s), 1));
-          if (++s == S::STAGES) {
+            for (int k = 0; k < S::BK / 32; ++k)
+              umma_i8_pair(d_tmem, ad + 2ull * k, bd + 2ull * k, idesc,
+                           (kb != 0 || k != 0) ? 1u : 0u);
+            umma_commit_both(bar(S::BAR_EMPTY + s));
+          }
+          __syncwarp();
+          if (++s == p.stages) {
             s = 0;
             ph ^= 1u;
           }
         }
-        if (ok) {
-          umma_commit_pair(mapa_shared(bar(S::BAR_TFULL + b), 0));
-          umma_commit_pair(mapa_shared(bar(S::BAR_TFULL + b), 1));
-        }
+        if (ok && issuer) umma_commit_both(bar(S::BAR_TFULL + b));
+        __syncwarp();
       }
-      umma_commit_pair(mapa_shared(bar(S::BAR_DRAIN), 0));
+      if (issuer) umma_commit_pair(mapa_shared(bar(S::BAR_DRAIN), 0));
       mbar_wait_drain(bar(S::BAR_DRAIN), 0);
     }
     __syncwarp();
   } else {
     // --------------------------------------------- epilogue (both CTAs)
-    constexpr int kOut = kGated ? BN / 2 : BN;          // output columns of a tile
-    constexpr int kCols = kOut / kEpiHalves;            // of which this warp's
-    constexpr int kChunks = kCols / 32;
     const int e = warp - 2;
     const int q = warp & 3;
-    const int c0 = (e / 4) * kCols;
+    // Output columns of a tile, and this warp's half of their 32-column chunks.
+    const int out_cols = kGated ? bn_cta : p.bn;
+    const int half = (out_cols / 32 + 1) / 2;
+    const int c0 = (e / 4) * half * 32;
+    const int chunks = e / 4 == 0 ? half : out_cols / 32 - half;
     EpilogueCtx<T> c;
     c.tmY = &tmY;
     c.tmR = &tmR;
@@ -551,9 +566,9 @@ __global__ void __launch_bounds__(Int8PairShape<BN>::THREADS, 1)
     c.M = p.M;
     c.N = p.N;
     c.has_residual = p.has_residual;
-    c.ebuf0 = base + S::OFF_EPI + e * kEpiBufs * kEpiBufBytes;
-    c.ebuf_ptr0 = base_ptr + S::OFF_EPI + e * kEpiBufs * kEpiBufBytes;
-    c.rbar0 = bar(S::BAR_RES + e * kEpiBufs);
+    c.ebuf0 = base + S::OFF_EPI + e * S::EPI_BUFS * kEpiBufBytes;
+    c.ebuf_ptr0 = base_ptr + S::OFF_EPI + e * S::EPI_BUFS * kEpiBufBytes;
+    c.rbar0 = bar(S::BAR_RES + e * S::EPI_BUFS);
     c.pol_stream = make_l2_policy_evict_first();
     float* const vec = reinterpret_cast<float*>(base_ptr + S::OFF_VEC + e * S::VEC_BYTES);
     uint32_t it = 0;
@@ -563,57 +578,68 @@ __global__ void __launch_bounds__(Int8PairShape<BN>::THREADS, 1)
       const uint32_t use_ph = (static_cast<uint32_t>(local) >> 1) & 1u;
       int mb, nb;
       int8_tile_coords(p, tile, mb, nb);
-      const int n0 = nb * kOut + c0;
+      const int n0 = nb * out_cols + c0;
       const int row_base = mb * 2 * S::BM + static_cast<int>(rank) * S::BM + q * 32;
       const int row = row_base + lane;
       const float sx = row < p.M ? p.sx[row] : 0.0f;
       __syncwarp();  // the previous tile's values are no longer read
-      int8_stage_vec(vec, p.sw, n0, kCols, p.N, lane);
-      int8_stage_vec(vec + 128, static_cast<const T*>(p.bias), n0, kCols, p.N, lane);
+      int8_stage_vec(vec, p.sw, n0, 32 * chunks, p.N, lane);
+      int8_stage_vec(vec + 128, static_cast<const T*>(p.bias), n0, 32 * chunks, p.N, lane);
       if (kGated) {
-        int8_stage_vec(vec + 256, p.sw2, n0, kCols, p.N, lane);
-        int8_stage_vec(vec + 384, static_cast<const T*>(p.bias2), n0, kCols, p.N, lane);
+        int8_stage_vec(vec + 256, p.sw2, n0, 32 * chunks, p.N, lane);
+        int8_stage_vec(vec + 384, static_cast<const T*>(p.bias2), n0, 32 * chunks, p.N, lane);
       }
       __syncwarp();
-      if (!mbar_wait(bar(S::BAR_TFULL + b), use_ph, abort_flag)) break;
+      const int live =
+          row_base < p.M && n0 < p.N ? min(chunks, (p.N - n0 + 31) / 32) : 0;
+      // A chunk's staging buffer is free, and its residual on the way, one chunk
+      // ahead (8192 x 14336 x 4096 with a residual: 363 us without).
+      if (live > 0) epi_chunk_begin<S::EPI_BUFS>(c, n0, row_base, lane, it);
+      if (!mbar_wait(bar(S::BAR_TFULL + b), use_ph, abort_flag)) {
+        if (live > 0) epi_chunk_drain<S::EPI_BUFS>(c, it);
+        break;
+      }
       tc_fence_after();
       const uint32_t tempty = mapa_shared(bar(S::BAR_TEMPTY + b), 0);
-      const uint32_t acc = tmem_base + static_cast<uint32_t>(b * BN) +
+      const uint32_t acc = tmem_base + static_cast<uint32_t>(b * S::MAX_BN) +
                            (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(c0);
-      const int live =
-          row_base < p.M && n0 < p.N ? min(kChunks, (p.N - n0 + 31) / 32) : 0;
       if (live == 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(tempty);
         continue;
       }
+      // (the first chunk's residual was asked for before the accumulator was ready)
       uint32_t r[32], u[32];
       tmem_ld_32x32b_x32(acc, r);
-      if (kGated) tmem_ld_32x32b_x32(acc + BN / 2, u);
+      if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(bn_cta), u);
       bool ok = true;
 #pragma unroll 1
       for (int ch = 0; ch < live; ++ch) {
-        epi_chunk_begin(c, n0 + 32 * ch, row_base, lane, it);
+        if (ch + 1 < live)
+          epi_chunk_begin<S::EPI_BUFS>(c, n0 + 32 * (ch + 1), row_base, lane, it + 1);
         tmem_wait_ld();
         float v[32], w[32];
         int8_scale(v, r, sx, vec + 32 * ch, vec + 128 + 32 * ch);
         if (kGated) int8_scale(w, u, sx, vec + 256 + 32 * ch, vec + 384 + 32 * ch);
         if (ch + 1 < live) {
           tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(32 * (ch + 1)), r);
-          if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(BN / 2 + 32 * (ch + 1)), u);
+          if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(bn_cta + 32 * (ch + 1)), u);
         } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(tempty);
         }
-        act_values(v, p.act);
+        act_values<sizeof(T) == 4>(v, p.act);
         if (kGated) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= w[j];
         }
-        if (!epi_chunk_store(c, v, n0 + 32 * ch, row_base, lane, it, abort_flag)) {
-          if (ch + 1 < live) tmem_wait_ld();
+        if (!epi_chunk_store<S::EPI_BUFS>(c, v, n0 + 32 * ch, row_base, lane, it, abort_flag)) {
+          if (ch + 1 < live) {
+            tmem_wait_ld();
+            epi_chunk_drain<S::EPI_BUFS>(c, it + 1);
+          }
           ok = false;
           break;
         }

@@ -41,9 +41,11 @@ int make_tmap_i8(CUtensorMap* m, const void* ptr, int64_t k, int64_t rows, int64
 
 // ---------------------------------------------------------- quantisation
 template <typename T, int THREADS>
-int launch_quantize(const QuantParams& p, cudaStream_t s) {
+int launch_quantize(const QuantParams& p, int sms, cudaStream_t s) {
+  // 1024 threads an SM, each CTA taking every grid'th row.
+  const int grid = std::min(p.M, sms * (1024 / THREADS));
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = launch_config(p.M, THREADS, 0, s, 1, attr);
+  cudaLaunchConfig_t cfg = launch_config(grid, THREADS, 0, s, 1, attr);
   cudaError_t e = cudaLaunchKernelEx(&cfg, dx::quantize_rows_kernel<T, THREADS>, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch quantize_rows_kernel");
@@ -52,14 +54,15 @@ int launch_quantize(const QuantParams& p, cudaStream_t s) {
 
 template <typename T>
 int quantize_typed(const QuantParams& p, int sms, cudaStream_t s) {
-  // Few rows: the latency of a row counts, one vector a thread; many: up to
-  // four vectors a thread, all loaded before the first is needed.
+  // Few rows: the latency of a row counts, one vector a thread; many: all that
+  // its registers hold, so that a row takes few threads and many are in flight.
+  constexpr int kRegs = dx::kQuantRegsOf<T>;
   const int vectors = (p.K + dx::kQuantVec - 1) / dx::kQuantVec;
-  const int threads = p.M <= 4 * sms ? vectors : (vectors + dx::kQuantRegs - 1) / dx::kQuantRegs;
-  if (threads <= 128) return launch_quantize<T, 128>(p, s);
-  if (threads <= 256) return launch_quantize<T, 256>(p, s);
-  if (threads <= 512) return launch_quantize<T, 512>(p, s);
-  return launch_quantize<T, 1024>(p, s);
+  const int threads = p.M <= 4 * sms ? vectors : (vectors + kRegs - 1) / kRegs;
+  if (threads <= 128) return launch_quantize<T, 128>(p, sms, s);
+  if (threads <= 256) return launch_quantize<T, 256>(p, sms, s);
+  if (threads <= 512) return launch_quantize<T, 512>(p, sms, s);
+  return launch_quantize<T, 1024>(p, sms, s);
 }
 
 int run_quantize(const void* X, void* Q, float* scale, int64_t M, int64_t K, int64_t ldx,
@@ -150,32 +153,46 @@ struct Int8Plan {
   bool pair = false;
   int bn = 256;               // pair
   int workers = 0;            // pair
-  int mn = 16, cluster = 1;   // tile
+  int mn = 16, cluster = 1, stages = 3;  // tile
 };
 
-// Tokens per tile: the fewest that hold M, up to 128.
-int int8_tile_mn(int64_t M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
-
+// Tile kernel: tokens per tile, CTAs per cluster and ring depth (B200; us, W in
+// L2).  Two CTAs fit an SM, so a wave is 2 * SMs tiles.
+//   tokens: the smallest of 16 / 32 / 64 / 128 whose tiles make one wave, then
+//   evened out.  M = 64, N = 4096: 10.0 with 32 a tile against 11.6 with 64;
+//   M = 512: 17.2 with 64, 19.3 with 128; M = 1024: 24.9 with 128 against 33.5
+//   with 64, which make two waves.
+//   cluster: as many CTAs as fill a wave, with some six K blocks each where there
+//   are that many.  M = 1, K = N = 4096: 6.3-6.6 for C = 5 to 8, 8.2 for 3, 11.6
+//   for 1; K = 14336: 11.3 for 7, 14.5 for 3; K = N = 1024: 4.0 for 4, 5.3 for 1.
+//   Beyond a wave it only costs: M = 16, N = 28672: 41 for 1, 45 for 2.
+//   ring: all of the SM's shared memory when each CTA has an SM to itself.
 Int8Plan int8_tile_plan(const Int8Problem& p, int sms) {
+  using S = Int8TileShape;
   Int8Plan pl;
-  pl.mn = int8_tile_mn(p.M);
-  const int64_t tiles = ((p.N + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128)) *
-                        ((p.M + pl.mn - 1) / pl.mn);
+  const int64_t n_tiles = (p.N + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128);
+  int64_t mn = 16;
+  while (mn < S::MAX_MN && mn < p.M &&
+         ((p.M + mn - 1) / mn > 1 && (mn < 32 || n_tiles * ((p.M + mn - 1) / mn) > 2 * sms)))
+    mn *= 2;
+  const int64_t m_tiles = (p.M + mn - 1) / mn;
+  pl.mn = static_cast<int>(round_up((p.M + m_tiles - 1) / m_tiles, 16));
+  const int64_t tiles = n_tiles * m_tiles;
   const int64_t k_blocks = (p.K + 127) / 128;
-  // Two CTAs an SM: split K while the CTAs fit, at least two blocks each.
-  for (int c = Int8TileShape<16>::MAX_CLUSTER; c > 1; --c)
-    if (tiles * c <= 2 * sms && k_blocks >= 2 * c) {
-      pl.cluster = c;
-      break;
-    }
+  const int64_t most = std::min<int64_t>(
+      std::min<int64_t>(S::MAX_CLUSTER, 2 * sms / tiles),
+      std::min<int64_t>(std::max<int64_t>(4, k_blocks / 6), k_blocks / 2));
+  pl.cluster = most >= (m_tiles > 1 ? 3 : 2) ? static_cast<int>(most) : 1;
+  const int room = tiles * pl.cluster <= sms ? S::FULL_SM : S::HALF_SM;
+  pl.stages = std::min<int>(S::MAX_STAGES, (room - S::smem_bytes(pl.mn, 0)) / S::stage_bytes(pl.mn));
   return pl;
 }
 
-template <int MN, typename T, bool G>
+template <typename T, bool G>
 int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
-  using S = Int8TileShape<MN>;
-  auto kern = dx::int8_tile_kernel<MN, T, G>;
-  int rc = ensure_smem_attr(dev, reinterpret_cast<const void*>(kern), S::SMEM_BYTES, true);
+  using S = Int8TileShape;
+  auto kern = dx::int8_tile_kernel<T, G>;
+  int rc = ensure_smem_attr(dev, reinterpret_cast<const void*>(kern), S::FULL_SM, true);
   if (rc) return rc;
   constexpr int NT = G ? 64 : 128;
   CUtensorMap tW, tW2, tX;
@@ -185,7 +202,7 @@ int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   } else {
     tW2 = tW;  // never read
   }
-  if ((rc = make_tmap_i8(&tX, pr.X, pr.K, pr.M, pr.ldx, MN, "X"))) return rc;
+  if ((rc = make_tmap_i8(&tX, pr.X, pr.K, pr.M, pr.ldx, static_cast<uint32_t>(pl.mn), "X"))) return rc;
   Int8Params p{};
   p.M = static_cast<int>(pr.M);
   p.N = static_cast<int>(pr.N);
@@ -200,16 +217,19 @@ int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.residual = pr.R;
   p.Y = pr.Y;
   p.act = pr.act;
+  p.mn = pl.mn;
+  p.stages = pl.stages;
   p.cluster = pl.cluster;
   p.w_early = pr.w_early ? 1 : 0;
   const int n_tiles = static_cast<int>((pr.N + NT - 1) / NT);
-  const int m_tiles = static_cast<int>((pr.M + MN - 1) / MN);
+  const int m_tiles = static_cast<int>((pr.M + pl.mn - 1) / pl.mn);
   set_plan("int8_tile%s tile=%dx%d stages=%d grid=%dx%d cluster=%d early=%d smem=%d",
-           G ? "_gated" : "", NT, MN, S::STAGES, n_tiles * pl.cluster, m_tiles, pl.cluster,
-           p.w_early, S::SMEM_BYTES);
+           G ? "_gated" : "", NT, pl.mn, pl.stages, n_tiles * pl.cluster, m_tiles, pl.cluster,
+           p.w_early, S::smem_bytes(pl.mn, pl.stages));
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = launch_config(n_tiles * pl.cluster, S::THREADS, S::SMEM_BYTES, pr.stream,
-                                         pl.cluster, attr);
+  cudaLaunchConfig_t cfg = launch_config(n_tiles * pl.cluster, S::THREADS,
+                                         S::smem_bytes(pl.mn, pl.stages), pr.stream, pl.cluster,
+                                         attr);
   cfg.gridDim.y = static_cast<unsigned>(m_tiles);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tW, tW2, tX, p);
   if (e == cudaSuccess) e = cudaGetLastError();
@@ -217,17 +237,17 @@ int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   return DX_OK;
 }
 
-template <int BN, typename T, bool G>
+template <typename T, bool G>
 int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
-  using S = Int8PairShape<BN>;
-  auto kern = dx::int8_pair_kernel<BN, T, G>;
+  using S = Int8PairShape;
+  auto kern = dx::int8_pair_kernel<T, G>;
   int rc = ensure_smem_attr(dev, reinterpret_cast<const void*>(kern), S::SMEM_BYTES, false);
   if (rc) return rc;
   CUtensorMap tA, tB, tB2, tY, tR;
   if ((rc = make_tmap_i8(&tA, pr.X, pr.K, pr.M, pr.ldx, 128, "X"))) return rc;
-  if ((rc = make_tmap_i8(&tB, pr.W, pr.K, pr.N, pr.ldw, BN / 2, "W"))) return rc;
+  if ((rc = make_tmap_i8(&tB, pr.W, pr.K, pr.N, pr.ldw, static_cast<uint32_t>(pl.bn / 2), "W"))) return rc;
   if (G) {
-    if ((rc = make_tmap_i8(&tB2, pr.W2, pr.K, pr.N, pr.ldw2, BN / 2, "W2"))) return rc;
+    if ((rc = make_tmap_i8(&tB2, pr.W2, pr.K, pr.N, pr.ldw2, static_cast<uint32_t>(pl.bn / 2), "W2"))) return rc;
   } else {
     tB2 = tB;  // never read
   }
@@ -241,8 +261,10 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   } else {
     tR = tY;  // never read
   }
-  constexpr int NT = G ? BN / 2 : BN;
+  const int NT = G ? pl.bn / 2 : pl.bn;
   Int8Params p{};
+  p.bn = pl.bn;
+  p.stages = std::min(S::MAX_STAGES, S::RING_BYTES / (S::A_BYTES + pl.bn / 2 * S::BK));
   p.M = static_cast<int>(pr.M);
   p.N = static_cast<int>(pr.N);
   p.k_blocks = static_cast<int>((pr.K + 127) / 128);
@@ -259,7 +281,7 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.group_m = pick_group_m(p.m_tiles, 256, (pr.K + 1) / 2);
   p.workers = std::min(pl.workers, p.num_tiles);
   set_plan("int8_pair%s tile=256x%d stages=%d grid=%d tiles=%d group_m=%d smem=%d",
-           G ? "_gated" : "", NT, S::STAGES, 2 * p.workers, p.num_tiles, p.group_m, S::SMEM_BYTES);
+           G ? "_gated" : "", NT, p.stages, 2 * p.workers, p.num_tiles, p.group_m, S::SMEM_BYTES);
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg =
       launch_config(2 * p.workers, S::THREADS, S::SMEM_BYTES, pr.stream, 2, attr);
@@ -269,48 +291,50 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   return DX_OK;
 }
 
-template <typename T, bool G>
-int dispatch_int8_tile(const Int8Problem& p, int dev, const Int8Plan& pl) {
-  switch (pl.mn) {
-    case 16: return launch_int8_tile<16, T, G>(p, dev, pl);
-    case 32: return launch_int8_tile<32, T, G>(p, dev, pl);
-    case 64: return launch_int8_tile<64, T, G>(p, dev, pl);
-    default: return launch_int8_tile<128, T, G>(p, dev, pl);
-  }
-}
-
-template <typename T, bool G>
-int dispatch_int8_pair(const Int8Problem& p, int dev, const Int8Plan& pl) {
-  if constexpr (!G) {
-    if (pl.bn == 128) return launch_int8_pair<128, T, G>(p, dev, pl);
-  }
-  return launch_int8_pair<256, T, G>(p, dev, pl);
-}
-
 template <bool G>
 int dispatch_int8(const Int8Problem& p, int dev, const Int8Plan& pl) {
   if (pl.pair)
-    return p.dtype == DX_DTYPE_F16 ? dispatch_int8_pair<__half, G>(p, dev, pl)
-                                   : dispatch_int8_pair<__nv_bfloat16, G>(p, dev, pl);
-  if (p.dtype == DX_DTYPE_F32) return dispatch_int8_tile<float, G>(p, dev, pl);
-  return p.dtype == DX_DTYPE_F16 ? dispatch_int8_tile<__half, G>(p, dev, pl)
-                                 : dispatch_int8_tile<__nv_bfloat16, G>(p, dev, pl);
+    return p.dtype == DX_DTYPE_F16 ? launch_int8_pair<__half, G>(p, dev, pl)
+                                   : launch_int8_pair<__nv_bfloat16, G>(p, dev, pl);
+  if (p.dtype == DX_DTYPE_F32) return launch_int8_tile<float, G>(p, dev, pl);
+  return p.dtype == DX_DTYPE_F16 ? launch_int8_tile<__half, G>(p, dev, pl)
+                                 : launch_int8_tile<__nv_bfloat16, G>(p, dev, pl);
 }
 
+// Accumulator columns of the pair kernel's tiles.  A wave of tiles takes about
+// max(bn + 134, 268) (a narrow tile is bound by its X rows: K = 4096, sustained,
+// us a wave: 8.0 at 128, 8.8 at 160, 9.6 at 192, 10.7 at 224, 11.6 at 256), and
+// the last tile's epilogue, about bn, is not overlapped.  M = N = K = 4096: 45 us
+// at 256 (4 waves), 47 at 192 (5), 56 at 128 (7); M = 512: 12.4 at 128, 15.4 at
+// 256, 18.1 at 64 (2 waves); M = 3000, N = 5000: 43.5 at 224, 46 at 256.
+int int8_pair_bn(const Int8Problem& p, int workers) {
+  const int step = p.gated ? 64 : 32, wide = p.gated ? 2 : 1;
+  const int64_t m_tiles = (p.M + 255) / 256;
+  int best = 256;
+  int64_t best_cost = -1;
+  for (int bn = 256; bn >= 64; bn -= step) {
+    const int64_t tiles = m_tiles * ((wide * p.N + bn - 1) / bn);
+    const int64_t cost = (tiles + workers - 1) / workers * std::max(bn + 134, 268) + bn;
+    if (best_cost < 0 || cost < best_cost) {
+      best_cost = cost;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+// Pairs from 65 tokens on (us): M = 128, K = N = 4096: 11.5 against 12.3 for the
+// tile kernel; M = 256: 11.2 against 13.8; M = 64: 10.9 against 10.0, and with
+// N = 14336 17.9 against 14.2.
 Int8Plan int8_plan(const Int8Problem& p, int dev, int sms) {
   Int8Plan pl = int8_tile_plan(p, sms);
   if (p.kernel == DX_KERNEL_DECODE || !int8_pair_eligible(p)) return pl;
+  if (p.kernel == DX_KERNEL_AUTO && p.M <= 64) return pl;
   const int slots = std::min(pair_slots<256, __nv_bfloat16>(dev, sms), sms / 2);
   if (slots < 1) return pl;
-  const int64_t m_tiles = (p.M + 255) / 256;
-  const int64_t tiles = m_tiles * ((p.N + (p.gated ? 127 : 255)) / (p.gated ? 128 : 256));
-  if (p.kernel == DX_KERNEL_UMMA || (p.M > 128 && tiles >= slots)) {
-    pl.pair = true;
-    pl.workers = slots;
-    const int64_t wide = (tiles + slots - 1) / slots;
-    const int64_t narrow = (m_tiles * ((p.N + 127) / 128) + slots - 1) / slots;
-    pl.bn = !p.gated && narrow < 2 * 0.8 * wide ? 128 : 256;
-  }
+  pl.pair = true;
+  pl.workers = slots;
+  pl.bn = int8_pair_bn(p, slots);
   return pl;
 }
 

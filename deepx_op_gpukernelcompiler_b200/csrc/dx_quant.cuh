@@ -5,17 +5,16 @@
 // the scale NaN (and q = 0), which makes every product with it NaN.
 //
 // Bound by memory: a row is read once into registers (rows of more than
-// kQuantRegs vectors a thread are read twice, the second time from L2), its
+// the threads' registers hold are read twice, the second time from L2), its
 // largest magnitude found on the integer bit patterns (ordered as the
 // magnitudes are, and a NaN stays the largest), and one byte a value written.
 //
-// The rounding is exact.  v = x * (127 / a) in fp32 is off by at most
-// 127 * 1.5 * 2^-23 < 3e-5, so the nearest integer of v is the right one
-// unless v lies within that of a half; those few values (|v - rint(v)| above
-// 0.4999) are rounded from the quotient in 64 bits, where 127 x is exact and a
-// quotient that is not a half differs from one by more than 2^-35.
-// Rows of 2^100 and more are scaled by 2^-64 first (exact) so that nothing
-// overflows.
+// The rounding is exact.  With c = 127 / a in fp32, x * c differs from the
+// quotient by at most 127 * 2^-24 + 2^-24 < 1e-5, so the integer nearest to it
+// is the right one unless x * c lies within that of a half; vectors with a value
+// that does (distance to its integer above 0.4999) are rounded again by the sign
+// of 127 x - (k + 1/2) a, k = floor(x * c), in 64 bits, where both products are
+// exact.  About eight instructions a value.
 #pragma once
 
 #include "dx_epilogue.cuh"
@@ -24,7 +23,11 @@
 namespace dx {
 
 constexpr int kQuantVec = 8;   // values a vector: one 16-byte load of a 16-bit type
-constexpr int kQuantRegs = 4;  // vectors of a row that a thread keeps in registers
+// 16-byte words of a row that a thread keeps in registers: 4 vectors of a 16-bit
+// type, 2 of fp32.
+constexpr int kQuantWords = 4;
+template <typename T>
+constexpr int kQuantRegsOf = kQuantWords * 2 / static_cast<int>(sizeof(T));
 
 struct QuantParams {
   const void* X;
@@ -81,37 +84,61 @@ __device__ __forceinline__ void quant_floats(const QuantVec<T>& v, float (&f)[kQ
   }
 }
 
+// The larger of m and the magnitudes of the vector, as bit patterns of T: of
+// two 16-bit values at once, in both halves of m.  A NaN is the largest.
 template <typename T>
 __device__ __forceinline__ uint32_t quant_max(uint32_t m, const QuantVec<T>& v) {
-  float f[kQuantVec];
-  quant_floats(v, f);
 #pragma unroll
-  for (int i = 0; i < kQuantVec; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  for (int i = 0; i < QuantVec<T>::kWords; ++i) {
+    if constexpr (sizeof(T) == 4)
+      m = max(m, v.w[i] & 0x7fffffffu);
+    else
+      m = __vmaxu2(m, v.w[i] & 0x7fff7fffu);
+  }
   return m;
 }
 
-// The nearest integer of 127 x / a; c = 127 / a in fp32.
-__device__ __forceinline__ int quant_one(float x, float a, float c) {
-  const float v = x * c;
-  // Adding 1.5 * 2^23 leaves the nearest integer in the low mantissa bits.
-  const float t = v + 12582912.0f;
-  int q = static_cast<int>(__float_as_uint(t)) - 0x4b400000;
-  if (fabsf(v - (t - 12582912.0f)) > 0.4999f)
-    q = static_cast<int>(rint(127.0 * static_cast<double>(x) / static_cast<double>(a)));
-  return q;
+// The fp32 bit pattern of a quant_max.
+template <typename T>
+__device__ __forceinline__ uint32_t quant_max_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) {
+    return m;
+  } else {
+    const float2 p = ElemTraits<T>::unpack2(max(m & 0xffffu, m >> 16));
+    return __float_as_uint(p.x) & 0x7fffffffu;
+  }
 }
 
+// 127 x / a of a vector, rounded; c = 127 / a in fp32, 0 for a row of zeros.
 template <typename T>
 __device__ __forceinline__ void quant_store(int8_t* q, int n, bool vec, const QuantVec<T>& x,
-                                            float pre, float a, float c) {
+                                            float a, float c) {
   float f[kQuantVec];
   quant_floats(x, f);
-  uint32_t b[2] = {0u, 0u};
+  uint32_t t[kQuantVec];
+  float off = 0.0f;
 #pragma unroll
   for (int i = 0; i < kQuantVec; ++i) {
-    const uint32_t v = static_cast<uint32_t>(quant_one(f[i] * pre, a, c)) & 0xffu;
-    b[i >> 2] |= v << (8 * (i & 3));
+    // Adding 1.5 * 2^23 leaves the nearest integer in the low mantissa bits.
+    const float r = fmaf(f[i], c, 12582912.0f);
+    off = fmaxf(off, fabsf(fmaf(f[i], c, 12582912.0f - r)));
+    t[i] = __float_as_uint(r);
   }
+  if (off > 0.4999f) {
+#pragma unroll
+    for (int i = 0; i < kQuantVec; ++i) {
+      const float k = floorf(f[i] * c);
+      const double d = 127.0 * static_cast<double>(f[i]) -
+                       (static_cast<double>(k) + 0.5) * static_cast<double>(a);
+      const int q0 = static_cast<int>(k);
+      t[i] = static_cast<uint32_t>(q0 + ((d > 0.0 || (d == 0.0 && (q0 & 1))) ? 1 : 0));
+    }
+  }
+  uint32_t b[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    b[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040),
+                       __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
   if (c == 0.0f) b[0] = b[1] = 0u;  // a row with an infinity or a NaN
   if (vec && n >= kQuantVec) {
     *reinterpret_cast<uint2*>(q) = make_uint2(b[0], b[1]);
@@ -122,56 +149,70 @@ __device__ __forceinline__ void quant_store(int8_t* q, int n, bool vec, const Qu
   }
 }
 
-// One row per CTA.
+// A row per CTA at a time, rows gridDim.x apart.  The next row's loads are issued
+// before this row's maximum is joined, so that they are in flight through the
+// barriers, the arithmetic and the stores.
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantParams p) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+    quantize_rows_kernel(const QuantParams p) {
   constexpr int kWarps = THREADS / 32;
-  __shared__ uint32_t s_max[kWarps];
+  constexpr int kQuantRegs = kQuantRegsOf<T>;
+  __shared__ uint32_t s_max[2][kWarps];
   grid_dependency_wait();
   grid_launch_dependents();
-  const long long row = blockIdx.x;
-  const T* const x = static_cast<const T*>(p.X) + row * p.ldx;
-  int8_t* const q = p.Q + row * p.ldq;
   const int vectors = (p.K + kQuantVec - 1) / kQuantVec;
   const bool vec = p.vec != 0;
-
-  QuantVec<T> f[kQuantRegs];
-  uint32_t m = 0;
+  const T* const X = static_cast<const T*>(p.X);
+  auto load_row = [&](long long row, QuantVec<T> (&f)[kQuantRegs]) {
 #pragma unroll
-  for (int r = 0; r < kQuantRegs; ++r) {
-    const int i = r * THREADS + static_cast<int>(threadIdx.x);
-    if (i < vectors) {
-      f[r] = quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec);
-      m = quant_max(m, f[r]);
+    for (int r = 0; r < kQuantRegs; ++r) {
+      const int i = r * THREADS + static_cast<int>(threadIdx.x);
+      if (i < vectors)
+        f[r] = quant_load(X + row * p.ldx + static_cast<long long>(i) * kQuantVec,
+                          p.K - i * kQuantVec, vec);
     }
-  }
-  for (int i = kQuantRegs * THREADS + static_cast<int>(threadIdx.x); i < vectors; i += THREADS)
-    m = quant_max(m, quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec));
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-  __syncthreads();
-  m = s_max[0];
+  };
+  QuantVec<T> next[kQuantRegs];
+  load_row(blockIdx.x, next);
+  int half = 0;
+  for (long long row = blockIdx.x; row < p.M; row += gridDim.x, half ^= 1) {
+    QuantVec<T> f[kQuantRegs];
+    uint32_t m = 0;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) m = max(m, s_max[w]);
+    for (int r = 0; r < kQuantRegs; ++r) {
+      f[r] = next[r];
+      if (r * THREADS + static_cast<int>(threadIdx.x) < vectors) m = quant_max(m, f[r]);
+    }
+    if (row + gridDim.x < p.M) load_row(row + gridDim.x, next);
+    const T* const x = X + row * p.ldx;
+    int8_t* const q = p.Q + row * p.ldq;
+    for (int i = kQuantRegs * THREADS + static_cast<int>(threadIdx.x); i < vectors; i += THREADS)
+      m = quant_max(m, quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec));
+    m = __reduce_max_sync(0xffffffffu, quant_max_bits<T>(m));
+    // Two arrays in turn: a warp may be a row ahead of one still reading.
+    if ((threadIdx.x & 31) == 0) s_max[half][threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = s_max[half][0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = max(m, s_max[half][w]);
 
-  const bool finite = m < 0x7f800000u;
-  const float top = fmaxf(__uint_as_float(finite ? m : 0u), 0x1p-100f);
-  if (threadIdx.x == 0)
-    p.scale[row] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
-  const float pre = top >= 0x1p100f ? 0x1p-64f : 1.0f;
-  const float a = top * pre;
-  const float c = finite ? __fdiv_rn(127.0f, a) : 0.0f;
+    const bool finite = m < 0x7f800000u;
+    const float top = fmaxf(__uint_as_float(finite ? m : 0u), 0x1p-100f);
+    if (threadIdx.x == 0)
+      p.scale[row] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
+    const float c = finite ? __fdiv_rn(127.0f, top) : 0.0f;
 #pragma unroll
-  for (int r = 0; r < kQuantRegs; ++r) {
-    const int i = r * THREADS + static_cast<int>(threadIdx.x);
-    if (i < vectors)
-      quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec, f[r], pre, a,
-                  c);
+    for (int r = 0; r < kQuantRegs; ++r) {
+      const int i = r * THREADS + static_cast<int>(threadIdx.x);
+      if (i < vectors)
+        quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec, f[r], top,
+                    c);
+    }
+    for (int i = kQuantRegs * THREADS + static_cast<int>(threadIdx.x); i < vectors; i += THREADS)
+      quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec,
+                  quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec),
+                  top, c);
   }
-  for (int i = kQuantRegs * THREADS + static_cast<int>(threadIdx.x); i < vectors; i += THREADS)
-    quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec,
-                quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec), pre,
-                a, c);
 }
 
 }  // namespace dx

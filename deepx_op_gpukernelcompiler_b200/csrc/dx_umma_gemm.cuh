@@ -170,11 +170,12 @@ struct EpilogueCtx {
 
 // Staging-buffer half of a 32-column chunk: waits until the store that last
 // used this buffer has read it, and starts the residual tile's TMA load.
-template <typename T>
+// With kAhead = 1 it is called one chunk ahead of the stores.
+template <int kBufs = kEpiBufs, int kAhead = kBufs - kEpiBufs, typename T>
 __device__ __forceinline__ void epi_chunk_begin(const EpilogueCtx<T>& c, int n_c, int row_base,
                                                 int lane, uint32_t it) {
-  const int buf = it % kEpiBufs;
-  if (lane == 0) bulk_wait_group_read<kEpiBufs - 1>();
+  const int buf = it % kBufs;
+  if (lane == 0) bulk_wait_group_read<kBufs - 1 - kAhead>();
   __syncwarp();
   if (c.has_residual && lane == 0) {
     const uint32_t rbar = c.rbar0 + 8u * buf;
@@ -206,22 +207,29 @@ __device__ __forceinline__ uint4 epi_load_bias(const EpilogueCtx<T>& c, int n0, 
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+// Waits for the residual load that epi_chunk_begin(it) started, when its chunk
+// will not be finished.
+template <int kBufs, typename T>
+__device__ __forceinline__ void epi_chunk_drain(const EpilogueCtx<T>& c, uint32_t it) {
+  if (c.has_residual) mbar_wait_drain(c.rbar0 + 8u * (it % kBufs), (it / kBufs) & 1u);
+}
+
 // The rest of a 32-column chunk whose values are final but for the residual:
 // adds it, converts, stages (64-byte swizzle) and TMA-stores.  Returns false if
 // the residual wait gave up.
-template <typename T>
+template <int kBufs = kEpiBufs, typename T>
 __device__ __forceinline__ bool epi_chunk_store(const EpilogueCtx<T>& c, float (&v)[32], int n_c,
                                                 int row_base, int lane, uint32_t& it,
                                                 volatile int* abort_flag) {
   using Tr = ElemTraits<T>;
-  const int buf = it % kEpiBufs;
+  const int buf = it % kBufs;
   const uint32_t ebuf = c.ebuf0 + buf * kEpiBufBytes;
   uint8_t* const ebp = c.ebuf_ptr0 + buf * kEpiBufBytes;
   const uint32_t row_off = static_cast<uint32_t>(lane) * 64u;
   const uint32_t row_sw = (static_cast<uint32_t>(lane) >> 1) & 3u;  // 64-byte swizzle phase
   if (c.has_residual) {
     const uint32_t rbar = c.rbar0 + 8u * buf;
-    const uint32_t par = (it / kEpiBufs) & 1u;
+    const uint32_t par = (it / kBufs) & 1u;
     if (!mbar_wait(rbar, par, abort_flag)) {
       mbar_wait_drain(rbar, par);  // the load still lands in this buffer
       return false;

@@ -94,84 +94,116 @@ def int8_rows(q: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
     return Int8Rows(q, scale.contiguous())
 
 
-def _pair(name: str, rows, K: int | None, n: int | None) -> tuple[torch.Tensor, torch.Tensor, int]:
-    """Checks an (int8 rows, scales) pair -> (q, scale, pitch)."""
+def _pair(name: str, rows, K: int | None, n: int | None) -> tuple:
+    """Checks an (int8 rows, scales) pair -> (q, scale, rows, K, pitch)."""
     if not isinstance(rows, tuple) or len(rows) != 2:
         raise TypeError(f"{name} must be a pair (int8 rows, float32 scales), see quantize_rows")
     q, scale = rows
-    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+    if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise ValueError(f"{name} must hold int8 rows and float32 scales, got {q.dtype} and "
                          f"{scale.dtype}")
-    _check_matrix(name, q, n, K)
-    if scale.dim() != 1 or scale.shape[0] != q.shape[0] or not scale.is_contiguous():
+    if q.dim() != 2:
+        raise ValueError(f"{name} must be 2-D, got shape {tuple(q.shape)}")
+    rows_, cols = q.shape
+    ld, unit = q.stride()
+    if (K is not None and cols != K) or (n is not None and rows_ != n) or unit != 1 or ld < cols:
+        _check_matrix(name, q, n, K)  # raises, unless the stride of a lone row or column is odd
+    if scale.dim() != 1 or scale.shape[0] != rows_ or not scale.is_contiguous():
         raise ValueError(f"{name} needs one contiguous scale per row, got {tuple(scale.shape)}")
-    ld = q.stride(0) if q.shape[0] > 1 else -(-q.shape[1] // 16) * 16
+    if rows_ <= 1:
+        ld = -(-cols // 16) * 16
     if ld % 16 or q.data_ptr() % 16:
         raise ValueError(f"{name}'s rows must start on 16 bytes (pitch {ld}): int8_rows(q, scale) "
                          f"lays them out")
-    return q, scale, ld
+    return q, scale, rows_, cols, ld
 
 
-def _vector(name: str, b: torch.Tensor | None, N: int) -> None:
-    if b is not None and (b.dim() != 1 or b.shape[0] != N or not b.is_contiguous()):
+def _float_or_pair(X, dtype):
+    """X of a product -> (x, dtype code, scale, M, K, pitch, output dtype)."""
+    if isinstance(X, torch.Tensor):
+        code = DTYPE_CODES.get(X.dtype)
+        if code is None:
+            raise ValueError(f"unsupported dtype {X.dtype}; expected float32, float16 or "
+                             f"bfloat16, or a pair (int8 rows, scales)")
+        _check_matrix("X", X, None, None)
+        M, K = X.shape
+        x, scale, ld, out_dtype = X, None, _ld(X), X.dtype if dtype is None else dtype
+    else:
+        x, scale, M, K, ld = _pair("X", X, None, None)
+        code, out_dtype = nat.DX_DTYPE_I8, torch.bfloat16 if dtype is None else dtype
+    if out_dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported output dtype {out_dtype}; expected float32, float16 or "
+                         f"bfloat16")
+    if K < 1:
+        raise ValueError("X must have at least one column")
+    return x, code, scale, M, K, ld, out_dtype
+
+
+def _kernel(kernel: str) -> int:
+    code = _KERNELS.get(kernel)
+    if code is None:
+        raise ValueError(f"unknown kernel {kernel!r}; expected one of {list(_KERNELS)}")
+    return code
+
+
+def _output(name: str, out, x: torch.Tensor, M: int, N: int, dtype: torch.dtype) -> torch.Tensor:
+    if x.device.type != "cuda":
+        raise ValueError(f"{name} runs on CUDA tensors only (the engine has no CPU path)")
+    if out is None:
+        return torch.empty((M, N), dtype=dtype, device=x.device)
+    _check_matrix("out", out, M, N)
+    _like("out", out, x, dtype)
+    return out
+
+
+def _like(name: str, t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype | None) -> None:
+    if dtype is not None and t.dtype is not dtype:
+        raise ValueError(f"{name} dtype {t.dtype} differs from the output dtype {dtype}")
+    if t.get_device() != x.get_device():
+        raise ValueError(f"{name} is on {t.device}, X is on {x.device}")
+
+
+def _vector(name: str, b: torch.Tensor | None, N: int, x: torch.Tensor, dtype: torch.dtype):
+    """Checks a bias -> its address (None without one)."""
+    if b is None:
+        return None
+    if b.dim() != 1 or b.shape[0] != N or not b.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of shape ({N},)")
+    _like(name, b, x, dtype)
+    return b.data_ptr()
 
 
-class _Call:
-    """The checks and arguments that both products share."""
+class _on:
+    """The device of x made current for a launch; `stream` is its current stream's handle."""
 
-    __slots__ = ("name", "x", "x_code", "x_scale", "M", "K", "ldx", "device", "dtype", "act",
-                 "kernel")
+    __slots__ = ("guard", "stream")
 
-    def __init__(self, name, X, dtype, activation, kernel):
-        self.act = activation_code(activation)
-        if kernel not in _KERNELS:
-            raise ValueError(f"unknown kernel {kernel!r}; expected one of {list(_KERNELS)}")
-        self.kernel = _KERNELS[kernel]
-        if isinstance(X, torch.Tensor):
-            if X.dtype not in DTYPE_CODES:
-                raise ValueError(f"unsupported dtype {X.dtype}; expected float32, float16 or "
-                                 f"bfloat16, or a pair (int8 rows, scales)")
-            _check_matrix("X", X, None, None)
-            self.x, self.x_scale, self.ldx = X, None, _ld(X)
-            self.x_code = DTYPE_CODES[X.dtype]
-            self.dtype = X.dtype if dtype is None else dtype
-        else:
-            self.x, self.x_scale, self.ldx = _pair("X", X, None, None)
-            self.x_code = nat.DX_DTYPE_I8
-            self.dtype = torch.bfloat16 if dtype is None else dtype
-        if self.dtype not in DTYPE_CODES:
-            raise ValueError(f"unsupported output dtype {self.dtype}; expected float32, float16 or "
-                             f"bfloat16")
-        self.M, self.K = self.x.shape
-        self.device = self.x.device
-        self.name = name
-        if self.K < 1:
-            raise ValueError("X must have at least one column")
+    def __init__(self, x: torch.Tensor):
+        index = x.get_device()
+        self.guard = None
+        if index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(index)
+        self.stream = torch.cuda.current_stream(index).cuda_stream
 
-    def check(self, typed, placed) -> None:
-        if self.device.type != "cuda":
-            raise ValueError(f"{self.name} runs on CUDA tensors only (the engine has no CPU path)")
-        for name, t in typed:
-            if t is not None and t.dtype != self.dtype:
-                raise ValueError(f"{name} dtype {t.dtype} differs from the output dtype "
-                                 f"{self.dtype}")
-        for name, t in typed + placed:
-            if t is not None and t.device != self.device:
-                raise ValueError(f"{name} is on {t.device}, X is on {self.device}")
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self.stream
 
-    def workspace(self) -> torch.Tensor | None:
-        # Of this call alone, from the allocator of the current stream or of the
-        # graph being captured: calls on other streams and other graphs cannot
-        # share it.
-        if self.x_scale is not None or self.M == 0:
-            return None
-        return torch.empty(nat.load().dx_int8_workspace_size(self.M, self.K), dtype=torch.uint8,
-                           device=self.device)
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
 
 
-def _ptr(t: torch.Tensor | None):
-    return t.data_ptr() if t is not None else None
+def _workspace(lib, x: torch.Tensor, x_scale, M: int, K: int):
+    # Of this call alone, from the allocator of the current stream or of the
+    # graph being captured: calls on other streams and other graphs cannot share
+    # it, and the allocator keeps it from others until the launches are done.
+    if x_scale is not None or M == 0:
+        return None, None, 0
+    space = torch.empty(lib.dx_int8_workspace_size(M, K), dtype=torch.uint8, device=x.device)
+    return space, space.data_ptr(), space.numel()
 
 
 def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
@@ -183,27 +215,28 @@ def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
     Int8Rows pair.  W: an Int8Rows pair [N, K] (quantize_weight).  Y has X's type,
     or `dtype` (bfloat16 by default where X is a pair); bias, residual and out
     have Y's."""
-    c = _Call("int8_linear", X, dtype, activation, kernel)
-    wq, ws, ldw = _pair("W", W, c.K, None)
-    N = wq.shape[0]
-    _vector("bias", bias, N)
+    act, kcode = activation_code(activation), _kernel(kernel)
+    x, x_code, x_scale, M, K, ldx, dtype = _float_or_pair(X, dtype)
+    wq, ws, N, _, ldw = _pair("W", W, K, None)
+    out = _output("int8_linear", out, x, M, N, dtype)
+    for name, t in (("W", wq), ("W's scale", ws), ("X's scale", x_scale)):
+        if t is not None:
+            _like(name, t, x, None)
+    b_ptr = _vector("bias", bias, N, x, dtype)
+    r_ptr, ldr = None, 0
     if residual is not None:
-        _check_matrix("residual", residual, c.M, N)
-    if out is None:
-        out = torch.empty((c.M, N), dtype=c.dtype, device=c.device)
-    else:
-        _check_matrix("out", out, c.M, N)
-    c.check([("bias", bias), ("residual", residual), ("out", out)],
-            [("W", wq), ("W's scale", ws), ("X's scale", c.x_scale)])
-    with torch.cuda.device(c.device):
-        space = c.workspace()
-        rc = nat.load().dx_int8_linear(
-            c.x.data_ptr(), c.x_code, _ptr(c.x_scale), wq.data_ptr(), ws.data_ptr(), _ptr(bias),
-            _ptr(residual), out.data_ptr(), c.M, N, c.K, c.ldx, ldw,
-            _ld(residual) if residual is not None else 0, _ld(out), DTYPE_CODES[c.dtype], c.act,
-            c.kernel, _ptr(space), space.numel() if space is not None else 0,
-            torch.cuda.current_stream(c.device).cuda_stream)
-    nat.check("dx_int8_linear", rc)
+        _check_matrix("residual", residual, M, N)
+        _like("residual", residual, x, dtype)
+        r_ptr, ldr = residual.data_ptr(), _ld(residual)
+    lib = nat.load()
+    with _on(x) as stream:
+        space, ws_ptr, ws_bytes = _workspace(lib, x, x_scale, M, K)
+        rc = lib.dx_int8_linear(
+            x.data_ptr(), x_code, x_scale.data_ptr() if x_scale is not None else None,
+            wq.data_ptr(), ws.data_ptr(), b_ptr, r_ptr, out.data_ptr(), M, N, K, ldx, ldw, ldr,
+            _ld(out), DTYPE_CODES[dtype], act, kcode, ws_ptr, ws_bytes, stream)
+    if rc:
+        nat.check("dx_int8_linear", rc)
     return out
 
 
@@ -213,28 +246,27 @@ def int8_gated_linear(X, Wg, Wu, bias_g: torch.Tensor | None = None,
                       kernel: str = "auto") -> torch.Tensor:
     """Y = act(X Wg^T + bias_g) * (X Wu^T + bias_u) on 8-bit operands, X read
     once for both weights (dx_int8_gated_linear).  Arguments as int8_linear."""
-    c = _Call("int8_gated_linear", X, dtype, activation, kernel)
-    gq, gs, ldg = _pair("Wg", Wg, c.K, None)
-    N = gq.shape[0]
-    uq, us, ldu = _pair("Wu", Wu, c.K, N)
-    _vector("bias_g", bias_g, N)
-    _vector("bias_u", bias_u, N)
-    if out is None:
-        out = torch.empty((c.M, N), dtype=c.dtype, device=c.device)
-    else:
-        _check_matrix("out", out, c.M, N)
-    c.check([("bias_g", bias_g), ("bias_u", bias_u), ("out", out)],
-            [("Wg", gq), ("Wg's scale", gs), ("Wu", uq), ("Wu's scale", us),
-             ("X's scale", c.x_scale)])
-    with torch.cuda.device(c.device):
-        space = c.workspace()
-        rc = nat.load().dx_int8_gated_linear(
-            c.x.data_ptr(), c.x_code, _ptr(c.x_scale), gq.data_ptr(), gs.data_ptr(), uq.data_ptr(),
-            us.data_ptr(), _ptr(bias_g), _ptr(bias_u), out.data_ptr(), c.M, N, c.K, c.ldx, ldg,
-            ldu, _ld(out), DTYPE_CODES[c.dtype], c.act, c.kernel, _ptr(space),
-            space.numel() if space is not None else 0,
-            torch.cuda.current_stream(c.device).cuda_stream)
-    nat.check("dx_int8_gated_linear", rc)
+    act, kcode = activation_code(activation), _kernel(kernel)
+    x, x_code, x_scale, M, K, ldx, dtype = _float_or_pair(X, dtype)
+    gq, gs, N, _, ldg = _pair("Wg", Wg, K, None)
+    uq, us, _, _, ldu = _pair("Wu", Wu, K, N)
+    out = _output("int8_gated_linear", out, x, M, N, dtype)
+    for name, t in (("Wg", gq), ("Wg's scale", gs), ("Wu", uq), ("Wu's scale", us),
+                    ("X's scale", x_scale)):
+        if t is not None:
+            _like(name, t, x, None)
+    bg_ptr = _vector("bias_g", bias_g, N, x, dtype)
+    bu_ptr = _vector("bias_u", bias_u, N, x, dtype)
+    lib = nat.load()
+    with _on(x) as stream:
+        space, ws_ptr, ws_bytes = _workspace(lib, x, x_scale, M, K)
+        rc = lib.dx_int8_gated_linear(
+            x.data_ptr(), x_code, x_scale.data_ptr() if x_scale is not None else None,
+            gq.data_ptr(), gs.data_ptr(), uq.data_ptr(), us.data_ptr(), bg_ptr, bu_ptr,
+            out.data_ptr(), M, N, K, ldx, ldg, ldu, _ld(out), DTYPE_CODES[dtype], act, kcode,
+            ws_ptr, ws_bytes, stream)
+    if rc:
+        nat.check("dx_int8_gated_linear", rc)
     return out
 
 
