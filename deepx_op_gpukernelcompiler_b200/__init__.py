@@ -9,7 +9,8 @@ copies overlapped with the fused launches), ``fused_gated_linear`` (the gated
 dual GEMM) and the FFN chains ``mlp_residual``, ``gated_ffn`` and
 ``two_layer_ffn``; the same layers on 8-bit integers with a scale per token and
 channel (``quantize_rows``, ``quantize_weight``, ``int8_rows``, ``int8_linear``,
-``int8_gated_linear``, ``int8_gated_ffn``).  Every compute call goes through the C ABI of
+``int8_gated_linear``, ``int8_gated_ffn``); and ``moe_ffn``, a whole
+mixture-of-experts layer for a few tokens.  Every compute call goes through the C ABI of
 ``libdeepx_fused.so`` (include/deepx_fused.h).
 """
 from .fusion import ACTIVATION_PT, FUSION_DB, classify
@@ -20,6 +21,7 @@ from .kernel_b200 import make_linear_kernel
 from .kvfunc import list_funcs, read_func
 from .linear import fused_gated_linear, fused_linear, fused_linear_host
 from .mlp import gated_ffn, mlp_residual, two_layer_ffn
+from .moe import moe_ffn
 
 __all__ = [
     "read_func", "list_funcs", "FUSION_DB", "classify", "ACTIVATION_PT",
@@ -28,5 +30,5 @@ __all__ = [
     "mlp_residual", "gated_ffn",
     "two_layer_ffn",
     "Int8Rows", "quantize_rows", "quantize_weight", "int8_rows", "int8_linear",
-    "int8_gated_linear", "int8_gated_ffn",
+    "int8_gated_linear", "int8_gated_ffn", "moe_ffn",
 ]

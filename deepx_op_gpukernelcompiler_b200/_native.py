@@ -86,6 +86,8 @@ SIGNATURES = {
     "dx_int8_gated_linear": (ctypes.c_int, [_vp, ctypes.c_int] + [_vp] * 8 + [_i64] * 7
                              + [ctypes.c_int] * 3 + [_vp, ctypes.c_size_t, _vp]),
     "dx_int8_workspace_size": (ctypes.c_size_t, [_i64, _i64]),
+    "dx_moe": (ctypes.c_int, [_vp, _vp]),
+    "dx_moe_workspace_size": (ctypes.c_size_t, [_i64] * 4),
     "dx_select_kernel": (ctypes.c_int, [_i64, _i64, _i64, ctypes.c_int]),
     "dx_copy_2d_async": (ctypes.c_int, [_vp, ctypes.c_size_t, _vp, ctypes.c_size_t,
                                         ctypes.c_size_t, ctypes.c_size_t, _vp]),
@@ -137,6 +139,18 @@ class RowReduceJob(ctypes.Structure):
         ("out_sym", ctypes.c_void_p),
         ("ldo", ctypes.c_int64),
     ]
+
+
+class MoeArgs(ctypes.Structure):
+    """ctypes mirror of ``dx_moe_args`` (include/deepx_fused.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("X", "Wr", "br", "Wg", "Wu", "Wo", "bg", "bu", "bo",
+                                                "R", "Y", "ids", "weights")]
+                + [(n, ctypes.c_int64) for n in ("T", "D", "H", "E", "top_k", "ldx", "ldwr", "ldg",
+                                                 "ldg_expert", "ldu", "ldu_expert", "ldo",
+                                                 "ldo_expert", "ldr", "ldy")]
+                + [(n, ctypes.c_int) for n in ("dtype", "act", "renormalize")]
+                + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)])
 
 
 _lock = threading.Lock()

@@ -1526,3 +1526,4 @@ extern "C" int dx_fused_linear_decode_noalloc(const void* X, const void* W, cons
 }
 
 #include "dx_int8_api.cuh"
+#include "dx_moe_api.cuh"

@@ -1,0 +1,789 @@
+// dx_moe.cuh — a mixture-of-experts layer for the few tokens of a serving step:
+//   l = x Wr + br;  the k experts of the largest l (ties: lowest number);
+//   w_e = exp(l_e) / sum of exp(l) over the chosen (or over all) experts;
+//   y = r + sum_e w_e ((act(x Wg_e + bg_e) * (x Wu_e + bu_e)) Wo_e + bo_e)
+// with T <= 64 tokens, E <= 256 experts, fp16 / bf16 weights as they lie in
+// memory (Wg, Wu [E][D][H], Wo [E][H][D]).
+//
+// Bound by the weights of the experts that some token chose, each read once.
+// Two launches:
+//
+//   moe_router_kernel  clusters of 8 CTAs, 8 tokens each: the CTAs split D, add
+//     their fp32 partial logits through distributed shared memory, and CTA i
+//     picks token i's experts.
+//   moe_experts_kernel  one CTA per SM, all resident (cooperative launch).
+//     Phase 1 computes h = act(gate) * up of every chosen expert, phase 2 the
+//     output; each phase's work units (tile x 64-deep K block) are dealt evenly
+//     and contiguously over the CTAs, so every SM streams the same bytes
+//     whatever the sizes.  As in the skinny-M decode kernel the operands are
+//     swapped: 128 weight columns are the MMA's rows (an MN-major operand, as W
+//     lies in memory) and the tokens its columns.  All tokens go through every
+//     chosen expert — the MMA has columns to spare, and no gathering is needed —
+//     and the epilogue uses a token's column only where the token chose the
+//     expert, so nothing of an expert (an infinity, a NaN) reaches other tokens.
+//     h is kept as a sum of two 16-bit values (hi + lo, 16 or 22 bits), both
+//     multiplied by Wo: the second product is as exact as with fp32 h, at no
+//     cost beside the weights' stream.
+//     A tile that several CTAs share leaves fp32 partial sums; when all are
+//     there the CTAs that end in the tile finish a share of its rows each,
+//     adding the partials in CTA order (results do not depend on timing).
+//     Between the phases the CTAs wait for one another, with the first weights
+//     of phase 2 already on their way.
+//
+// Every wait is bounded, as in dx_umma_gemm.cuh.
+#pragma once
+
+#include "dx_epilogue.cuh"
+#include "dx_ptx.cuh"
+
+namespace dx {
+
+constexpr int kMoeMaxT = 64;
+constexpr int kMoeMaxE = 256;
+constexpr int kMoeMaxTop = 32;
+
+// ---------------------------------------------------------------- router
+constexpr int kRouterThreads = 512;
+constexpr int kRouterTokens = 8;  // tokens of a cluster = its CTAs
+constexpr int kRouterRows = 256;  // rows of Wr per step
+
+struct MoeRouterParams {
+  const void* X;
+  const void* Wr;  // [D][E], pitch ldwr
+  const void* br;  // [E] or nullptr
+  long long ldx, ldwr;
+  int T, D, E, top, renormalize;
+  int* ids;        // [T][top]
+  float* weights;  // [T][top]
+  int* counters;   // zeroed for moe_experts_kernel
+  int num_counters;
+};
+
+// Unsigned key in the order of the floats (a NaN sorts by its sign and bits).
+__device__ __forceinline__ uint32_t moe_key(float f) {
+  const uint32_t u = __float_as_uint(f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRouterParams p) {
+  using Tr = ElemTraits<T>;
+  __shared__ __align__(16) float s_x[kRouterRows][kRouterTokens];
+  __shared__ float s_part[kRouterThreads * kRouterTokens];  // [row group][token][expert]
+  __shared__ float s_sum[kRouterTokens][kMoeMaxE];
+  __shared__ float s_logit[kMoeMaxE];
+  const int tid = static_cast<int>(threadIdx.x);
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int t0 = static_cast<int>(blockIdx.x) / kRouterTokens * kRouterTokens;
+  const int tokens = min(kRouterTokens, p.T - t0);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (blockIdx.x == 0)
+    for (int i = tid; i < p.num_counters; i += kRouterThreads) p.counters[i] = 0;
+
+  // Threads as row groups x experts; each sums its rows for all tokens.
+  const int ep = (p.E + 31) / 32 * 32;
+  const int groups = kRouterThreads / ep;
+  const int e = tid % ep, kg = tid / ep;
+  const bool live = kg < groups && e < p.E;
+  const int slice = (p.D + kRouterTokens - 1) / kRouterTokens;
+  const int k_begin = rank * slice, k_end = min(p.D, k_begin + slice);
+  const T* const X = static_cast<const T*>(p.X);
+  const T* const Wr = static_cast<const T*>(p.Wr);
+  float acc[kRouterTokens];
+#pragma unroll
+  for (int t = 0; t < kRouterTokens; ++t) acc[t] = 0.0f;
+  for (int k0 = k_begin; k0 < k_end; k0 += kRouterRows) {
+    const int rows = min(kRouterRows, k_end - k0);
+    __syncthreads();
+    for (int i = tid; i < kRouterRows * kRouterTokens; i += kRouterThreads) {
+      const int t = i / kRouterRows, k = i % kRouterRows;
+      s_x[k][t] = t < tokens && k < rows ? Tr::to_float(X[(t0 + t) * p.ldx + k0 + k]) : 0.0f;
+    }
+    __syncthreads();
+    if (live) {
+      constexpr int kBatch = 16;  // rows whose loads are issued together
+      for (int k = kg; k < rows; k += kBatch * groups) {
+        float w[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int kk = k + i * groups;
+          w[i] = kk < rows ? Tr::to_float(Wr[(k0 + kk) * p.ldwr + e]) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int kk = k + i * groups;
+          if (kk < rows) {
+            const float4 a = *reinterpret_cast<const float4*>(&s_x[kk][0]);
+            const float4 b = *reinterpret_cast<const float4*>(&s_x[kk][4]);
+            acc[0] = fmaf(a.x, w[i], acc[0]);
+            acc[1] = fmaf(a.y, w[i], acc[1]);
+            acc[2] = fmaf(a.z, w[i], acc[2]);
+            acc[3] = fmaf(a.w, w[i], acc[3]);
+            acc[4] = fmaf(b.x, w[i], acc[4]);
+            acc[5] = fmaf(b.y, w[i], acc[5]);
+            acc[6] = fmaf(b.z, w[i], acc[6]);
+            acc[7] = fmaf(b.w, w[i], acc[7]);
+          }
+        }
+      }
+    }
+  }
+  if (kg < groups) {
+#pragma unroll
+    for (int t = 0; t < kRouterTokens; ++t) s_part[(kg * kRouterTokens + t) * ep + e] = acc[t];
+  }
+  __syncthreads();
+  for (int i = tid; i < kRouterTokens * ep; i += kRouterThreads) {
+    const int t = i / ep, ee = i % ep;
+    float s = 0.0f;
+    for (int g = 0; g < groups; ++g) s += s_part[(g * kRouterTokens + t) * ep + ee];
+    s_sum[t][ee] = s;
+  }
+  cluster_sync();
+  const int token = t0 + rank;
+  if (rank < tokens) {
+    for (int i = tid; i < p.E; i += kRouterThreads) {
+      float s = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kRouterTokens; ++c)
+        s += ld_shared_cluster_f32(
+            mapa_shared(smem_u32(&s_sum[rank][i]), static_cast<uint32_t>(c)));
+      if (p.br != nullptr) s += Tr::to_float(static_cast<const T*>(p.br)[i]);
+      s_logit[i] = s;
+    }
+  }
+  cluster_sync();  // no CTA leaves while its sums are read
+  if (rank >= tokens || tid >= 32) return;
+
+  // One warp: lane l holds experts l, l + 32, ...
+  constexpr int kPer = kMoeMaxE / 32;
+  uint32_t key[kPer];  // 0: absent or taken (no float's key is 0 but a NaN's)
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int ee = i * 32 + tid;
+    key[i] = ee < p.E ? max(moe_key(s_logit[ee]), 1u) : 0u;
+  }
+  float top_logit = 0.0f, sum = 0.0f, mine = 0.0f;
+  int my_id = 0;
+  for (int j = 0; j < p.top; ++j) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    uint32_t at = kMoeMaxE;
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; --i)
+      if (key[i] == best) at = static_cast<uint32_t>(i * 32 + tid);
+    const int id = static_cast<int>(__reduce_min_sync(0xffffffffu, at));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i * 32 + tid == id) key[i] = 0;
+    const float l = s_logit[id];
+    if (j == 0) top_logit = l;
+    const float x = expf(l - top_logit);
+    sum += x;
+    if (tid == j) {
+      mine = x;
+      my_id = id;
+    }
+  }
+  if (!p.renormalize) {
+    sum = 0.0f;
+    for (int ee = tid; ee < p.E; ee += 32) sum += expf(s_logit[ee] - top_logit);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  if (tid < p.top) {
+    p.ids[token * p.top + tid] = my_id;
+    p.weights[token * p.top + tid] = mine / sum;
+  }
+}
+
+// --------------------------------------------------------------- experts
+struct MoeParams {
+  int T, D, H, E, top, act;
+  int kb_d, nt_h;  // phase 1: 64-deep blocks of D, 128-column tiles of H
+  int kb_h, nt_d;  // phase 2: 64-deep blocks of H, 256-column tiles of D
+  int mn;          // tokens padded to a multiple of 16
+  int stages;
+  const int* ids;
+  const float* weights;
+  const void *bg, *bu, *bo;  // [E][H], [E][H], [E][D] or nullptr
+  const void* residual;
+  long long ldr;
+  void* Y;
+  long long ldy;
+  void *h_hi, *h_lo;  // [chosen experts][T][H]
+  float* partials;    // [CTA][first / later tile][2][T][128]
+  int* counters;      // [2 phases][CTA] tile arrivals, then the phase barrier; zero before
+};
+
+struct MoeShape {
+  static constexpr int BK = 64;
+  static constexpr int BOX_BYTES = 64 * BK * 2;  // [64 k x 64 n]
+  static constexpr int W_BYTES = 4 * BOX_BYTES;  // 256 columns
+  static constexpr int MAX_STAGES = 6;
+  static constexpr int THREADS = 192;
+  // Behind the ring (W tiles, then token tiles):
+  static constexpr int OFF_IDS = 0;                                    // [T * top]
+  static constexpr int OFF_WTS = OFF_IDS + kMoeMaxT * kMoeMaxTop * 4;  // [T * top]
+  static constexpr int OFF_MASK = OFF_WTS + kMoeMaxT * kMoeMaxTop * 4;  // [E] tokens, 64 bits
+  static constexpr int OFF_LIST = OFF_MASK + kMoeMaxE * 8;             // chosen experts
+  static constexpr int OFF_ROWW = OFF_LIST + kMoeMaxE * 4;             // [2][64] weights of a run
+  static constexpr int OFF_BAR = OFF_ROWW + 2 * kMoeMaxT * 4;
+  static constexpr int BAR_FULL = 0;
+  static constexpr int BAR_EMPTY = MAX_STAGES;
+  static constexpr int BAR_TFULL = 2 * MAX_STAGES;
+  static constexpr int BAR_TEMPTY = BAR_TFULL + 2;
+  static constexpr int BAR_DRAIN = BAR_TEMPTY + 2;
+  static constexpr int NUM_BARS = BAR_DRAIN + 1;
+  static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;  // tmem base, abort flag, experts, ok
+  static constexpr int TAIL_BYTES = OFF_MISC + 32;
+  static constexpr int stage_bytes(int mn) { return W_BYTES + 2 * mn * BK * 2; }
+  static constexpr int smem_bytes(int mn, int stages) {
+    return 1024 + stages * stage_bytes(mn) + TAIL_BYTES;
+  }
+  static constexpr int max_stages(int mn) {
+    const int n = (227 * 1024 - smem_bytes(mn, 0)) / stage_bytes(mn);
+    return n < MAX_STAGES ? n : MAX_STAGES;
+  }
+};
+
+// A run of K blocks that one accumulator collects: one tile's (phase 1), or one
+// tile's of one expert (phase 2).
+struct MoeRun {
+  int tile, a, kb0, len;  // a: index into the chosen experts
+  int u;                  // its first unit
+};
+
+// One phase's units and this CTA's share of them.
+struct MoePhase {
+  int units, ctas;  // CTAs that have units
+  int per_tile;     // units of a tile
+  int nt, kb;       // phase 1: tiles of an expert; K blocks of an expert's product
+  int u0, u1;
+  bool second;
+
+  __device__ __forceinline__ int begin(int g) const {
+    return static_cast<int>(static_cast<long long>(g) * units / ctas);
+  }
+  __device__ __forceinline__ int cta_of(int u) const {
+    int g = static_cast<int>(static_cast<long long>(u) * ctas / units);
+    while (g + 1 < ctas && begin(g + 1) <= u) ++g;
+    return g;
+  }
+  // The unit's tile, expert index and K block.
+  __device__ __forceinline__ void unit(int u, int& tile, int& a, int& kb_) const {
+    tile = u / per_tile;
+    const int r = u - tile * per_tile;
+    if (second) {
+      a = r / kb;
+      kb_ = r - a * kb;
+    } else {
+      a = tile / nt;
+      kb_ = r;
+    }
+  }
+  __device__ __forceinline__ bool run(int u, MoeRun& r) const {
+    if (u >= u1) return false;
+    r.u = u;
+    unit(u, r.tile, r.a, r.kb0);
+    r.len = min(kb - r.kb0, u1 - u);
+    return true;
+  }
+};
+
+__device__ __forceinline__ MoePhase moe_phase(const MoeParams& p, int chosen, bool second) {
+  MoePhase f;
+  f.second = second;
+  f.kb = second ? p.kb_h : p.kb_d;
+  f.nt = p.nt_h;
+  f.per_tile = second ? chosen * p.kb_h : p.kb_d;
+  f.units = second ? p.nt_d * f.per_tile : chosen * p.nt_h * f.per_tile;
+  f.ctas = min(static_cast<int>(gridDim.x), f.units);
+  const int g = static_cast<int>(blockIdx.x);
+  f.u0 = g < f.ctas ? f.begin(g) : 0;
+  f.u1 = g < f.ctas ? f.begin(g + 1) : 0;
+  return f;
+}
+
+// Bounded wait until *ctr reaches `target` (every CTA of the launch is resident).
+__device__ __forceinline__ bool moe_wait(const int* ctr, int target, volatile int* abort_flag) {
+  const uint64_t t0 = global_timer_ns();
+  uint32_t spins = 0;
+  while (*reinterpret_cast<const volatile int*>(ctr) < target) {
+    __nanosleep(20);
+    if ((++spins & 63u) == 0) {
+      if (*abort_flag) return false;
+      if (global_timer_ns() - t0 > kWaitLimitNs) {
+        *abort_flag = 1;
+        report_timeout();
+        return false;
+      }
+    }
+  }
+  __threadfence();
+  return true;
+}
+
+// h of token m in column n of chosen expert a: stored as hi + lo.
+template <typename T>
+__device__ __forceinline__ void moe_store_h(const MoeParams& p, int a, int m, int n, float gate,
+                                            float up, float bg, float bu) {
+  using Tr = ElemTraits<T>;
+  float v[1] = {gate + bg};
+  act_values<false>(v, p.act);
+  const float h = v[0] * (up + bu);
+  const long long i = (static_cast<long long>(a) * p.T + m) * p.H + n;
+  const T hi = Tr::from_float(h);
+  // (an infinite hi has no lo: inf - inf)
+  const float rest = h - Tr::to_float(hi);
+  static_cast<T*>(p.h_hi)[i] = hi;
+  static_cast<T*>(p.h_lo)[i] = Tr::from_float(rest - rest == 0.0f ? rest : 0.0f);
+}
+
+template <int MN, typename T>
+__global__ void __launch_bounds__(MoeShape::THREADS, 1)
+    moe_experts_kernel(const __grid_constant__ CUtensorMap tmG,
+                       const __grid_constant__ CUtensorMap tmU,
+                       const __grid_constant__ CUtensorMap tmO,
+                       const __grid_constant__ CUtensorMap tmX,
+                       const __grid_constant__ CUtensorMap tmHi,
+                       const __grid_constant__ CUtensorMap tmLo, const MoeParams p) {
+  using S = MoeShape;
+  using Tr = ElemTraits<T>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw_u32 = smem_u32(smem_raw);
+  const uint32_t base = (raw_u32 + 1023u) & ~1023u;
+  uint8_t* const base_ptr = smem_raw + (base - raw_u32);
+  const int stages = p.stages;
+  const uint32_t t_bytes = static_cast<uint32_t>(p.mn) * S::BK * 2;  // one token tile
+  const uint32_t sW = base;
+  const uint32_t sT = base + static_cast<uint32_t>(stages) * S::W_BYTES;
+  const uint32_t tail = static_cast<uint32_t>(stages) * (S::W_BYTES + 2 * t_bytes);
+  uint8_t* const tail_ptr = base_ptr + tail;
+  const uint32_t bars = base + tail + S::OFF_BAR;
+  int* const s_ids = reinterpret_cast<int*>(tail_ptr + S::OFF_IDS);
+  float* const s_wts = reinterpret_cast<float*>(tail_ptr + S::OFF_WTS);
+  uint32_t* const s_mask = reinterpret_cast<uint32_t*>(tail_ptr + S::OFF_MASK);
+  int* const s_list = reinterpret_cast<int*>(tail_ptr + S::OFF_LIST);
+  float* const s_roww = reinterpret_cast<float*>(tail_ptr + S::OFF_ROWW);
+  uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(tail_ptr + S::OFF_MISC);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tail_ptr + S::OFF_MISC + 4);
+  int* const s_chosen = reinterpret_cast<int*>(tail_ptr + S::OFF_MISC + 8);
+  volatile int* const s_ok = reinterpret_cast<volatile int*>(tail_ptr + S::OFF_MISC + 12);
+  auto bar = [bars](int i) { return bars + 8u * static_cast<uint32_t>(i); };
+  constexpr uint32_t kTmemCols = 4 * MN < 32 ? 32 : 4 * MN;  // two buffers x two halves
+
+  const int tid = static_cast<int>(threadIdx.x);
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int lane = tid & 31;
+  const int g = static_cast<int>(blockIdx.x);
+
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(bar(S::BAR_FULL + s), 1);
+      mbar_init(bar(S::BAR_EMPTY + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(S::BAR_TFULL + b), 1);
+      mbar_init(bar(S::BAR_TEMPTY + b), 4);
+    }
+    mbar_init(bar(S::BAR_DRAIN), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmG);
+    tma_prefetch_desc(&tmU);
+    tma_prefetch_desc(&tmO);
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmHi);
+    tma_prefetch_desc(&tmLo);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_word), kTmemCols);
+    tmem_relinquish();
+  }
+  for (int i = tid; i < 2 * p.E; i += S::THREADS) s_mask[i] = 0;
+  // The routing, the zeroed counters and X come from launches before this one.
+  grid_dependency_wait();
+  const int pairs = p.T * p.top;
+  __syncthreads();
+  for (int i = tid; i < pairs; i += S::THREADS) {
+    const int e = p.ids[i], t = i / p.top;
+    s_ids[i] = e;
+    s_wts[i] = p.weights[i];
+    atomicOr(&s_mask[2 * e + (t >> 5)], 1u << (t & 31));
+  }
+  __syncthreads();
+  if (warp == 0) {  // the chosen experts in order of their numbers
+    int n = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + lane;
+      const bool c = e < p.E && (s_mask[2 * e] | s_mask[2 * e + 1]) != 0;
+      const uint32_t vote = __ballot_sync(0xffffffffu, c);
+      if (c) s_list[n + __popc(vote & ((1u << lane) - 1u))] = e;
+      n += __popc(vote);
+    }
+    if (lane == 0) *s_chosen = n;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_word;
+  const int chosen = *s_chosen;
+  int* const barrier_ctr = p.counters + 2 * gridDim.x;
+
+  if (warp == 0) {
+    // ------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const uint64_t pol = make_l2_policy_evict_first();
+      const uint64_t keep = make_l2_policy_evict_last();
+      uint32_t issued = 0;
+      bool ok = true;
+      auto load_w = [&](int ph, int u, const MoePhase& f, int s) {
+        int tile, a, kb;
+        f.unit(u, tile, a, kb);
+        const int e = s_list[a];
+        const uint32_t fb = bar(S::BAR_FULL + s);
+        const uint32_t dst = sW + s * S::W_BYTES;
+        if (ph == 0) {
+          const int n = (tile - a * f.nt) * 128;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tma_load_3d_hint(j < 2 ? &tmG : &tmU, dst + j * S::BOX_BYTES, fb, n + 64 * (j & 1),
+                             kb * S::BK, e, pol);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tma_load_3d_hint(&tmO, dst + j * S::BOX_BYTES, fb, tile * 256 + 64 * j, kb * S::BK, e,
+                             pol);
+        }
+      };
+      auto load_t = [&](int ph, int u, const MoePhase& f, int s) {
+        int tile, a, kb;
+        f.unit(u, tile, a, kb);
+        const uint32_t fb = bar(S::BAR_FULL + s);
+        const uint32_t dst = sT + static_cast<uint32_t>(s) * 2 * t_bytes;
+        if (ph == 0) {
+          tma_load_2d_hint(&tmX, dst, fb, kb * S::BK, 0, keep);
+        } else {
+          tma_load_2d_hint(&tmHi, dst, fb, kb * S::BK, a * p.T, keep);
+          tma_load_2d_hint(&tmLo, dst + t_bytes, fb, kb * S::BK, a * p.T, keep);
+        }
+      };
+      for (int ph = 0; ok && ph < 2; ++ph) {
+        const MoePhase f = moe_phase(p, chosen, ph != 0);
+        const uint32_t bytes = S::W_BYTES + (ph != 0 ? 2 * t_bytes : t_bytes);
+        int u = f.u0;
+        auto start = [&](int unit) {  // the unit's stage, its weights on their way
+          const int s = static_cast<int>(issued % stages);
+          if (!mbar_wait(bar(S::BAR_EMPTY + s), ((issued / stages) & 1u) ^ 1u, abort_flag))
+            return false;
+          mbar_arrive_expect_tx(bar(S::BAR_FULL + s), bytes);
+          load_w(ph, unit, f, s);
+          ++issued;
+          return true;
+        };
+        if (ph != 0) {
+          // A ring of phase 2's weights before every h is written.
+          const uint32_t first = issued;
+          const int early = min(stages, f.u1 - f.u0);
+          int n = 0;
+          while (n < early && start(u + n)) ++n;
+          ok = n == early && moe_wait(barrier_ctr, static_cast<int>(gridDim.x), abort_flag);
+          fence_proxy_async_global();
+          // (also when giving up, so that the started stages complete)
+          for (int i = 0; i < n; ++i)
+            load_t(ph, u + i, f, static_cast<int>((first + i) % stages));
+          u += n;
+        }
+        for (; ok && u < f.u1; ++u) {
+          ok = start(u);
+          if (ok) load_t(ph, u, f, static_cast<int>((issued - 1) % stages));
+        }
+      }
+      // Loads in flight land before the shared memory is released.
+      const uint32_t n_drain = min(issued, static_cast<uint32_t>(stages));
+      for (uint32_t i = issued - n_drain; i < issued; ++i)
+        mbar_wait_drain(bar(S::BAR_FULL + static_cast<int>(i % stages)), (i / stages) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------- MMA issuer
+    const uint32_t idesc = umma_idesc_f16(Tr::kIsBf16, 128, p.mn, true, false);
+    const bool issuer = elect_one();
+    int s = 0, local = 0;
+    uint32_t par = 0;
+    bool ok = true;
+    for (int ph = 0; ok && ph < 2; ++ph) {
+      const MoePhase f = moe_phase(p, chosen, ph != 0);
+      MoeRun r;
+      for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
+        const int b = local & 1;
+        if (!mbar_wait_warp(bar(S::BAR_TEMPTY + b), ((static_cast<uint32_t>(local) >> 1) & 1u) ^ 1u,
+                            abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(b * 2 * MN);
+        for (int i = 0; i < r.len; ++i) {
+          if (!mbar_wait_warp(bar(S::BAR_FULL + s), par, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (issuer) {
+            const uint64_t td = smem_desc_sw128(sT + static_cast<uint32_t>(s) * 2 * t_bytes, 16, 1024);
+            const uint64_t lo = smem_desc_sw128(sT + static_cast<uint32_t>(s) * 2 * t_bytes + t_bytes,
+                                                16, 1024);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              // 128 columns of W: MN-major, two 64-wide groups one box apart,
+              // 8-row K groups 1024 B apart; +2048 B per K = 16 step.
+              const uint64_t wd =
+                  smem_desc_sw128(sW + s * S::W_BYTES + h * 2 * S::BOX_BYTES, S::BOX_BYTES, 1024);
+              const uint32_t dh = d + static_cast<uint32_t>(h * MN);
+#pragma unroll
+              for (int k = 0; k < S::BK / 16; ++k)
+                umma_f16(dh, wd + 128ull * k, td + 2ull * k, idesc, (i != 0 || k != 0) ? 1u : 0u);
+              if (ph != 0) {
+#pragma unroll
+                for (int k = 0; k < S::BK / 16; ++k)
+                  umma_f16(dh, wd + 128ull * k, lo + 2ull * k, idesc, 1u);
+              }
+            }
+            umma_commit(bar(S::BAR_EMPTY + s));
+          }
+          __syncwarp();
+          if (++s == stages) {
+            s = 0;
+            par ^= 1u;
+          }
+        }
+        if (ok && issuer) umma_commit(bar(S::BAR_TFULL + b));
+        __syncwarp();
+      }
+    }
+    // Every MMA issued so far completes before TMEM can be freed.
+    if (issuer) umma_commit(bar(S::BAR_DRAIN));
+    mbar_wait_drain(bar(S::BAR_DRAIN), 0);
+    __syncwarp();
+  } else {
+    // --------------------------------------------------------- epilogue
+    const int q = warp & 3;
+    const int et = tid - 64;
+    const int n = q * 32 + lane;  // column within a 128-column half
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const T* const bg = static_cast<const T*>(p.bg);
+    const T* const bu = static_cast<const T*>(p.bu);
+    const T* const bo = static_cast<const T*>(p.bo);
+    int local = 0;
+    bool ok = true;
+    // This CTA's partial sums of its first (0) or a later (1) tile, and another's.
+    auto part = [&](int cta, int slot, int h, int m) {
+      return p.partials +
+             ((static_cast<long long>(cta * 2 + slot) * 2 + h) * p.T + m) * 128;
+    };
+    // Publishes are complete: counts this CTA in for the tile, and where it is the
+    // CTA's last tile waits for the others.  Afterwards [first, last] are the CTAs
+    // of the tile, `share` of `shares` this CTA's part of finishing it (-1: none).
+    int first = 0, last = 0, share = -1, shares = 1;
+    auto join = [&](const MoePhase& f, int tile) {
+      const int us = tile * f.per_tile, ue = us + f.per_tile;
+      first = f.cta_of(us);
+      last = f.cta_of(ue - 1);
+      const bool mine = f.u1 <= ue;  // this CTA ends in the tile
+      shares = last - first + (f.begin(last + 1) == ue ? 1 : 0);
+      share = mine ? g - first : -1;
+      __threadfence();
+      named_bar_sync(1, 128);
+      if (et == 0) {
+        int* const ctr = p.counters + (f.second ? gridDim.x : 0) + first;
+        atomicAdd(ctr, 1);
+        *s_ok = mine ? (moe_wait(ctr, last - first + 1, abort_flag) ? 1 : 0) : 1;
+      }
+      named_bar_sync(1, 128);
+      __threadfence();
+      return *s_ok != 0;
+    };
+    // The tile's partial sum of (half h, token m), in CTA order.
+    auto total = [&](const MoePhase& f, int tile, int h, int m) {
+      float sum = 0.0f;
+      int c = first;
+      for (; c + 3 <= last; c += 4) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i] = __ldcg(part(c + i, f.begin(c + i) / f.per_tile == tile ? 0 : 1, h, m) + n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += v[i];
+      }
+      for (; c <= last; ++c)
+        sum += __ldcg(part(c, f.begin(c) / f.per_tile == tile ? 0 : 1, h, m) + n);
+      return sum;
+    };
+
+    {  // ---- phase 1: h
+      const MoePhase f = moe_phase(p, chosen, false);
+      MoeRun r;
+      for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
+        const int b = local & 1;
+        const int e = s_list[r.a];
+        const int col = (r.tile - r.a * f.nt) * 128 + n;
+        const bool live = col < p.H;
+        const unsigned long long mask =
+            s_mask[2 * e] | (static_cast<unsigned long long>(s_mask[2 * e + 1]) << 32);
+        const long long bi = static_cast<long long>(e) * p.H + col;
+        const float vg = bg != nullptr && live ? Tr::to_float(bg[bi]) : 0.0f;
+        const float vu = bu != nullptr && live ? Tr::to_float(bu[bi]) : 0.0f;
+        // (the vote keeps the four warps together where a wait gives up)
+        ok = named_bar_all(1, 128, mbar_wait(bar(S::BAR_TFULL + b),
+                                             (static_cast<uint32_t>(local) >> 1) & 1u, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = lane_addr + static_cast<uint32_t>(b * 2 * MN);
+        const bool whole = r.len == f.per_tile;
+        const int slot = f.u0 / f.per_tile == r.tile ? 0 : 1;
+#pragma unroll 1
+        for (int mc = 0; mc < p.T; mc += 16) {
+          uint32_t a0[16], a1[16];
+          tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(mc), a0);
+          tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(MN + mc), a1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int m = mc + j;
+            if (m < p.T && ((mask >> m) & 1u)) {
+              const float ga = __uint_as_float(a0[j]), up = __uint_as_float(a1[j]);
+              if (!whole) {
+                part(g, slot, 0, m)[n] = ga;
+                part(g, slot, 1, m)[n] = up;
+              } else if (live) {
+                moe_store_h<T>(p, r.a, m, col, ga, up, vg, vu);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(S::BAR_TEMPTY + b));
+        if (!whole) {
+          ok = join(f, r.tile);
+          if (ok && share >= 0) {
+            int i = 0;
+            for (unsigned long long left = mask; left != 0; left &= left - 1, ++i) {
+              if (i % shares != share) continue;
+              const int m = __ffsll(static_cast<long long>(left)) - 1;
+              const float ga = total(f, r.tile, 0, m), up = total(f, r.tile, 1, m);
+              if (live) moe_store_h<T>(p, r.a, m, col, ga, up, vg, vu);
+            }
+          }
+        }
+      }
+    }
+    // Everything this CTA wrote of h, before any CTA reads it by TMA.
+    fence_proxy_async_global();
+    __threadfence();
+    named_bar_sync(1, 128);
+    if (et == 0 && ok) atomicAdd(barrier_ctr, 1);
+
+    {  // ---- phase 2: the output
+      const MoePhase f = moe_phase(p, chosen, true);
+      T* const Y = static_cast<T*>(p.Y);
+      const T* const res = static_cast<const T*>(p.residual);
+      float y[2][MN];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < MN; ++m) y[h][m] = 0.0f;
+      MoeRun r;
+      for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
+        const int b = local & 1;
+        const int e = s_list[r.a];
+        const int col = r.tile * 256 + n;
+        const unsigned long long mask =
+            s_mask[2 * e] | (static_cast<unsigned long long>(s_mask[2 * e + 1]) << 32);
+        // The tokens' weights for this expert.
+        float* const roww = s_roww + b * kMoeMaxT;
+        if (et < p.T) {
+          float w = 0.0f;
+          for (int j = 0; j < p.top; ++j)
+            if (s_ids[et * p.top + j] == e) w = s_wts[et * p.top + j];
+          roww[et] = w;
+        }
+        float vb[2] = {0.0f, 0.0f};
+        if (bo != nullptr && r.kb0 == 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (col + 128 * h < p.D)
+              vb[h] = Tr::to_float(bo[static_cast<long long>(e) * p.D + col + 128 * h]);
+        }
+        ok = named_bar_all(1, 128, mbar_wait(bar(S::BAR_TFULL + b),
+                                             (static_cast<uint32_t>(local) >> 1) & 1u, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = lane_addr + static_cast<uint32_t>(b * 2 * MN);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int mc = 0; mc < MN; mc += 16) {
+            if (mc < p.T) {
+              uint32_t v[16];
+              tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(h * MN + mc), v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if ((mask >> (mc + j)) & 1u)
+                  y[h][mc + j] = fmaf(roww[mc + j], __uint_as_float(v[j]) + vb[h], y[h][mc + j]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(S::BAR_TEMPTY + b));
+        // The CTA's last run of this tile?
+        const int us = r.tile * f.per_tile, ue = us + f.per_tile;
+        if (u + r.len < ue && u + r.len < f.u1) continue;
+        auto finish = [&](int h, int m, float sum) {
+          const int c = col + 128 * h;
+          if (c >= p.D) return;
+          if (res != nullptr) sum += Tr::to_float(res[m * p.ldr + c]);
+          Y[m * p.ldy + c] = Tr::from_float(sum);
+        };
+        const bool whole = f.u0 <= us && f.u1 >= ue;
+        const int slot = f.u0 / f.per_tile == r.tile ? 0 : 1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int m = 0; m < MN; ++m) {
+            if (m < p.T) {
+              if (whole)
+                finish(h, m, y[h][m]);
+              else
+                part(g, slot, h, m)[n] = y[h][m];
+            }
+            y[h][m] = 0.0f;
+          }
+        if (!whole) {
+          ok = join(f, r.tile);
+          if (ok && share >= 0)
+            for (int i = share; i < 2 * p.T; i += shares)
+              finish(i & 1, i >> 1, total(f, r.tile, i & 1, i >> 1));
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+}  // namespace dx

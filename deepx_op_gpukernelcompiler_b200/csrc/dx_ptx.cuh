@@ -152,6 +152,17 @@ __device__ __forceinline__ void tma_load_2d_hint(const CUtensorMap* m, uint32_t 
       : "memory");
 }
 
+// 3-D tiled load (box depth 1 in z), with an L2 eviction-priority policy.
+__device__ __forceinline__ void tma_load_3d_hint(const CUtensorMap* m, uint32_t dst, uint32_t bar,
+                                                 int32_t x, int32_t y, int32_t z,
+                                                 uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+
 // CTA-pair form: the copy lands in this CTA's shared memory and signals the
 // mbarrier at `bar`, a shared::cluster address that may be the pair
 // leader's barrier.  Reads only this GPU's global memory.
@@ -239,6 +250,20 @@ __device__ __forceinline__ void bulk_load_g2s(uint32_t dst, const void* src, uin
 
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
+// named_bar_sync that returns whether `pred` held in every thread.
+__device__ __forceinline__ bool named_bar_all(uint32_t id, uint32_t nthreads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %3, 0;\n\t"
+      "bar.red.and.pred p, %1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(nthreads), "r"(pred ? 1u : 0u)
+      : "memory");
+  return r != 0;
 }
 
 // --------------------------------------------------------------- clusters

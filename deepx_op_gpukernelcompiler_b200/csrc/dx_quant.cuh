@@ -9,12 +9,17 @@
 // largest magnitude found on the integer bit patterns (ordered as the
 // magnitudes are, and a NaN stays the largest), and one byte a value written.
 //
-// The rounding is exact.  With c = 127 / a in fp32, x * c differs from the
-// quotient by at most 127 * 2^-24 + 2^-24 < 1e-5, so the integer nearest to it
-// is the right one unless x * c lies within that of a half; vectors with a value
-// that does (distance to its integer above 0.4999) are rounded again by the sign
-// of 127 x - (k + 1/2) a, k = floor(x * c), in 64 bits, where both products are
-// exact.  About eight instructions a value.
+// The rounding is exact.  With c = 127 / a in fp32, x c is off by 2^-23 of the
+// quotient; one residual step, x c + (127 x - x c a) / a, leaves a half exactly a
+// half and anything else within 2^-24.  Between 16-bit values a quotient that is
+// not a half differs from one by more than 2^-20 of itself (127 x / a - (n + 1/2) =
+// (254 X - (2n + 1) 2^j A) / (2^(j+1) A) with integers X, A < 2^11), so adding
+// 1.5 * 2^23 rounds it as the exact quotient.  fp32 values can lie closer: those
+// within 1e-4 of a half are decided by the sign of 127 x - (k + 1/2) a in 64 bits,
+// where both products are exact.  127 x and a are taken times 2^-8, so that rows
+// near the end of bf16's range do not overflow.  Deciding the halves of 16-bit
+// rows in 64 bits too cost 21 instructions a value and 109 us for 8192 x 14336
+// (bf16 rows hold many exact halves).
 #pragma once
 
 #include "dx_epilogue.cuh"
@@ -109,29 +114,53 @@ __device__ __forceinline__ uint32_t quant_max_bits(uint32_t m) {
   }
 }
 
-// 127 x / a of a vector, rounded; c = 127 / a in fp32, 0 for a row of zeros.
+// What turns a row's values into integers.
+struct QuantRow {
+  float c;      // 127 / a; 0 for a row with an infinity or a NaN
+  float a;      // 2^-8 a
+  float inv_a;  // 1 / (2^-8 a)
+};
+
+__device__ __forceinline__ QuantRow quant_row(float top, bool finite) {
+  QuantRow r;
+  r.c = finite ? __fdiv_rn(127.0f, top) : 0.0f;
+  r.a = top * 0x1p-8f;
+  r.inv_a = __frcp_rn(r.a);
+  return r;
+}
+
+// The integers nearest to 127 x / a of a vector, stored as bytes.
 template <typename T>
 __device__ __forceinline__ void quant_store(int8_t* q, int n, bool vec, const QuantVec<T>& x,
-                                            float a, float c) {
+                                            const QuantRow& row) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the integer ends up in the low bits
   float f[kQuantVec];
   quant_floats(x, f);
   uint32_t t[kQuantVec];
-  float off = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kQuantVec; ++i) {
-    // Adding 1.5 * 2^23 leaves the nearest integer in the low mantissa bits.
-    const float r = fmaf(f[i], c, 12582912.0f);
-    off = fmaxf(off, fabsf(fmaf(f[i], c, 12582912.0f - r)));
-    t[i] = __float_as_uint(r);
-  }
-  if (off > 0.4999f) {
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < kQuantVec; ++i) {
-      const float k = floorf(f[i] * c);
-      const double d = 127.0 * static_cast<double>(f[i]) -
-                       (static_cast<double>(k) + 0.5) * static_cast<double>(a);
-      const int q0 = static_cast<int>(k);
-      t[i] = static_cast<uint32_t>(q0 + ((d > 0.0 || (d == 0.0 && (q0 & 1))) ? 1 : 0));
+      const float v = f[i] * row.c;
+      const float rest = fmaf(-v, row.a, f[i] * (127.0f * 0x1p-8f));
+      t[i] = __float_as_uint(fmaf(rest, row.inv_a, v) + kMagic);
+    }
+  } else {
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kQuantVec; ++i) {
+      const float r = fmaf(f[i], row.c, kMagic);
+      off = fmaxf(off, fabsf(fmaf(f[i], row.c, kMagic - r)));
+      t[i] = __float_as_uint(r);
+    }
+    if (off > 0.4999f) {
+#pragma unroll
+      for (int i = 0; i < kQuantVec; ++i) {
+        const float k = floorf(f[i] * row.c);
+        const double d = (127.0 / 256.0) * static_cast<double>(f[i]) -
+                         (static_cast<double>(k) + 0.5) * static_cast<double>(row.a);
+        const int q0 = static_cast<int>(k);
+        t[i] = static_cast<uint32_t>(q0 + ((d > 0.0 || (d == 0.0 && (q0 & 1))) ? 1 : 0));
+      }
     }
   }
   uint32_t b[2];
@@ -139,7 +168,7 @@ __device__ __forceinline__ void quant_store(int8_t* q, int n, bool vec, const Qu
   for (int i = 0; i < 2; ++i)
     b[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040),
                        __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
-  if (c == 0.0f) b[0] = b[1] = 0u;  // a row with an infinity or a NaN
+  if (row.c == 0.0f) b[0] = b[1] = 0u;  // a row with an infinity or a NaN
   if (vec && n >= kQuantVec) {
     *reinterpret_cast<uint2*>(q) = make_uint2(b[0], b[1]);
   } else {
@@ -200,18 +229,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     const float top = fmaxf(__uint_as_float(finite ? m : 0u), 0x1p-100f);
     if (threadIdx.x == 0)
       p.scale[row] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
-    const float c = finite ? __fdiv_rn(127.0f, top) : 0.0f;
+    const QuantRow qr = quant_row(top, finite);
 #pragma unroll
     for (int r = 0; r < kQuantRegs; ++r) {
       const int i = r * THREADS + static_cast<int>(threadIdx.x);
       if (i < vectors)
-        quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec, f[r], top,
-                    c);
+        quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec, f[r], qr);
     }
     for (int i = kQuantRegs * THREADS + static_cast<int>(threadIdx.x); i < vectors; i += THREADS)
       quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec,
                   quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec),
-                  top, c);
+                  qr);
   }
 }
 

@@ -328,6 +328,38 @@ int dx_int8_gated_linear(const void* X, int x_dtype, const float* x_scale, const
 size_t dx_int8_workspace_size(int64_t M, int64_t K);
 
 /*
+ * A mixture-of-experts layer for the tokens of a serving step (the reference
+ * lists its chain, `moe_ffn`, as multi_kernel and never runs it):
+ *   l = X Wr + br; each token's top_k experts by l, ties to the lowest number
+ *   w_e = exp(l_e) / (sum over the chosen experts, or over all: renormalize = 0)
+ *   Y = R + sum_e w_e ((act(X Wg[e] + bg[e]) * (X Wu[e] + bu[e])) Wo[e] + bo[e])
+ * in two launches that read the weights of each chosen expert once.  fp16/bf16;
+ * 0 <= T <= 64 tokens, E <= 256 experts, top_k <= min(E, 32), D and H multiples
+ * of 8 up to 65536.  X [T, D] (pitch ldx); Wr [D, E] (ldwr); Wg, Wu [E, D, H] and
+ * Wo [E, H, D] with row pitches ldg, ldu, ldo and expert pitches l*_expert; br
+ * [E], bg, bu [E, H], bo [E, D], R [T, D] (ldr) may be NULL.  Y [T, D] (ldy) may
+ * be R.  ids [T, top_k] and weights [T, top_k] receive the routing, largest
+ * first.  X and the expert weights: 16-byte-aligned, pitches multiples of 8.
+ * What an expert computes reaches only the tokens that chose it.  workspace:
+ * 256-byte-aligned, dx_moe_workspace_size() bytes, no initial value, used by no
+ * other call meanwhile.  The second launch is cooperative.
+ */
+typedef struct dx_moe_args {
+  const void *X, *Wr, *br, *Wg, *Wu, *Wo, *bg, *bu, *bo, *R;
+  void* Y;
+  int* ids;
+  float* weights;
+  int64_t T, D, H, E, top_k;
+  int64_t ldx, ldwr, ldg, ldg_expert, ldu, ldu_expert, ldo, ldo_expert, ldr, ldy;
+  int dtype, act, renormalize;
+  void* workspace;
+  size_t workspace_bytes;
+} dx_moe_args;
+
+int dx_moe(const dx_moe_args* args, void* stream);
+size_t dx_moe_workspace_size(int64_t T, int64_t H, int64_t E, int64_t top_k);
+
+/*
  * Plans — the compile-then-call runtime of the reference design docs: the
  * compile step fixes shape, dtype and op sequence
  * (doc/kvlang-to-tilelang-interface.md:60-77,100-129) and the runtime calls
