@@ -327,20 +327,18 @@ __device__ __forceinline__ bool moe_wait(const int* ctr, int target, volatile in
   return true;
 }
 
-// h of token m in column n of chosen expert a: stored as hi + lo.
+// h as hi + lo of type T.
 template <typename T>
-__device__ __forceinline__ void moe_store_h(const MoeParams& p, int a, int m, int n, float gate,
-                                            float up, float bg, float bu) {
+__device__ __forceinline__ void moe_split(float h, T& hi, T& lo) {
   using Tr = ElemTraits<T>;
-  float v[1] = {gate + bg};
-  act_values<false>(v, p.act);
-  const float h = v[0] * (up + bu);
-  const long long i = (static_cast<long long>(a) * p.T + m) * p.H + n;
-  const T hi = Tr::from_float(h);
-  // (an infinite hi has no lo: inf - inf)
+  hi = Tr::from_float(h);
   const float rest = h - Tr::to_float(hi);
-  static_cast<T*>(p.h_hi)[i] = hi;
-  static_cast<T*>(p.h_lo)[i] = Tr::from_float(rest - rest == 0.0f ? rest : 0.0f);
+  lo = Tr::from_float(rest - rest == 0.0f ? rest : 0.0f);  // an infinite hi has no lo
+}
+
+template <typename T>
+__device__ __forceinline__ float moe_bias(const T* b, long long i) {
+  return b != nullptr ? ElemTraits<T>::to_float(b[i]) : 0.0f;
 }
 
 template <int MN, typename T>
@@ -580,50 +578,71 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
     const T* const bg = static_cast<const T*>(p.bg);
     const T* const bu = static_cast<const T*>(p.bu);
     const T* const bo = static_cast<const T*>(p.bo);
+    T* const h_hi = static_cast<T*>(p.h_hi);
+    T* const h_lo = static_cast<T*>(p.h_lo);
     int local = 0;
     bool ok = true;
-    // This CTA's partial sums of its first (0) or a later (1) tile, and another's.
-    auto part = [&](int cta, int slot, int h, int m) {
-      return p.partials +
-             ((static_cast<long long>(cta * 2 + slot) * 2 + h) * p.T + m) * 128;
+    auto chosen_by = [&](int e) {  // the tokens of expert e
+      return s_mask[2 * e] | (static_cast<unsigned long long>(s_mask[2 * e + 1]) << 32);
     };
-    // Publishes are complete: counts this CTA in for the tile, and where it is the
-    // CTA's last tile waits for the others.  Afterwards [first, last] are the CTAs
-    // of the tile, `share` of `shares` this CTA's part of finishing it (-1: none).
-    int first = 0, last = 0, share = -1, shares = 1;
-    auto join = [&](const MoePhase& f, int tile) {
+    // Partial sums of a CTA's first tile (slot 0) or of its last (slot 1): [2][T][128].
+    const long long slot_floats = static_cast<long long>(2 * p.T) * 128;
+    auto part = [&](int cta, int slot) { return p.partials + (cta * 2 + slot) * slot_floats; };
+    // The tile whose partial sums this CTA has just written: `peers` CTAs from
+    // `first` on have a share of it, `sum` points at the first one's, and this CTA
+    // finishes every shares'th row from `share` on (-1: none).  Counts the CTA in;
+    // where the tile is its last one, waits until all are there.
+    const float* sum = nullptr;
+    int first = 0, peers = 1, share = 0, shares = 1;
+    auto join = [&](const MoePhase& f, int tile, int slot) {
       const int us = tile * f.per_tile, ue = us + f.per_tile;
-      first = f.cta_of(us);
-      last = f.cta_of(ue - 1);
-      const bool mine = f.u1 <= ue;  // this CTA ends in the tile
-      shares = last - first + (f.begin(last + 1) == ue ? 1 : 0);
-      share = mine ? g - first : -1;
+      const bool whole = f.u0 <= us && f.u1 >= ue;
+      first = g;
+      peers = shares = 1;
+      share = 0;
+      if (!whole) {
+        first = f.cta_of(us);
+        const int last = f.cta_of(ue - 1);
+        peers = last - first + 1;
+        shares = last - first + (f.begin(last + 1) == ue ? 1 : 0);
+        share = f.u1 <= ue ? g - first : -1;
+      }
+      // (a CTA that starts inside the tile has it as its first tile)
+      sum = part(first, first == g ? slot : (f.begin(first) / f.per_tile == tile ? 0 : 1));
       __threadfence();
       named_bar_sync(1, 128);
+      if (whole) return true;
       if (et == 0) {
         int* const ctr = p.counters + (f.second ? gridDim.x : 0) + first;
         atomicAdd(ctr, 1);
-        *s_ok = mine ? (moe_wait(ctr, last - first + 1, abort_flag) ? 1 : 0) : 1;
+        *s_ok = share < 0 || moe_wait(ctr, peers, abort_flag) ? 1 : 0;
       }
       named_bar_sync(1, 128);
       __threadfence();
       return *s_ok != 0;
     };
-    // The tile's partial sum of (half h, token m), in CTA order.
-    auto total = [&](const MoePhase& f, int tile, int h, int m) {
-      float sum = 0.0f;
-      int c = first;
-      for (; c + 3 <= last; c += 4) {
-        float v[4];
+    // Columns 4 lane .. 4 lane + 3 of row `row` of the tile, added in CTA order.
+    auto row_sum = [&](int row) {
+      const long long at = static_cast<long long>(row) * 128 + 4 * lane;
+      float4 t = __ldcg(reinterpret_cast<const float4*>(sum + at));
+      const float* const next = part(first + 1, 0) + at;
+#pragma unroll 1
+      for (int i = 0; i < peers - 1; i += 8) {
+        float4 v[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[i] = __ldcg(part(c + i, f.begin(c + i) / f.per_tile == tile ? 0 : 1, h, m) + n);
+        for (int k = 0; k < 8; ++k)
+          v[k] = i + k < peers - 1
+                     ? __ldcg(reinterpret_cast<const float4*>(next + 2 * slot_floats * (i + k)))
+                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += v[i];
+        for (int k = 0; k < 8; ++k) {
+          t.x += v[k].x;
+          t.y += v[k].y;
+          t.z += v[k].z;
+          t.w += v[k].w;
+        }
       }
-      for (; c <= last; ++c)
-        sum += __ldcg(part(c, f.begin(c) / f.per_tile == tile ? 0 : 1, h, m) + n);
-      return sum;
+      return t;
     };
 
     {  // ---- phase 1: h
@@ -632,55 +651,85 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
       for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
         const int b = local & 1;
         const int e = s_list[r.a];
-        const int col = (r.tile - r.a * f.nt) * 128 + n;
-        const bool live = col < p.H;
-        const unsigned long long mask =
-            s_mask[2 * e] | (static_cast<unsigned long long>(s_mask[2 * e + 1]) << 32);
-        const long long bi = static_cast<long long>(e) * p.H + col;
-        const float vg = bg != nullptr && live ? Tr::to_float(bg[bi]) : 0.0f;
-        const float vu = bu != nullptr && live ? Tr::to_float(bu[bi]) : 0.0f;
+        const int col0 = (r.tile - r.a * f.nt) * 128;
+        const unsigned long long mask = chosen_by(e);
+        const bool whole = r.len == f.per_tile;
+        const int slot = f.u0 / f.per_tile == r.tile ? 0 : 1;
+        const bool live = col0 + n < p.H;
+        float vg = 0.0f, vu = 0.0f;
+        if (whole && live) {
+          vg = moe_bias(bg, static_cast<long long>(e) * p.H + col0 + n);
+          vu = moe_bias(bu, static_cast<long long>(e) * p.H + col0 + n);
+        }
         // (the vote keeps the four warps together where a wait gives up)
         ok = named_bar_all(1, 128, mbar_wait(bar(S::BAR_TFULL + b),
                                              (static_cast<uint32_t>(local) >> 1) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t acc = lane_addr + static_cast<uint32_t>(b * 2 * MN);
-        const bool whole = r.len == f.per_tile;
-        const int slot = f.u0 / f.per_tile == r.tile ? 0 : 1;
 #pragma unroll 1
         for (int mc = 0; mc < p.T; mc += 16) {
+          const uint32_t some = static_cast<uint32_t>(mask >> mc) & 0xffffu;
+          if (some == 0) continue;
           uint32_t a0[16], a1[16];
           tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(mc), a0);
           tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(MN + mc), a1);
           tmem_wait_ld();
+          if (!whole) {
+            float* const to = part(g, slot) + mc * 128 + n;
+            float* const to1 = to + p.T * 128;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int m = mc + j;
-            if (m < p.T && ((mask >> m) & 1u)) {
-              const float ga = __uint_as_float(a0[j]), up = __uint_as_float(a1[j]);
-              if (!whole) {
-                part(g, slot, 0, m)[n] = ga;
-                part(g, slot, 1, m)[n] = up;
-              } else if (live) {
-                moe_store_h<T>(p, r.a, m, col, ga, up, vg, vu);
+            for (int j = 0; j < 16; ++j)
+              if ((some >> j) & 1u) {
+                to[j * 128] = __uint_as_float(a0[j]);
+                to1[j * 128] = __uint_as_float(a1[j]);
               }
-            }
+          } else {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(a0[j]) + vg;
+            act_values<false>(v, p.act);
+            const long long at = (static_cast<long long>(r.a) * p.T + mc) * p.H + col0 + n;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (((some >> j) & 1u) && live) {
+                T hi, lo;
+                moe_split(v[j] * (__uint_as_float(a1[j]) + vu), hi, lo);
+                h_hi[at + static_cast<long long>(j) * p.H] = hi;
+                h_lo[at + static_cast<long long>(j) * p.H] = lo;
+              }
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(S::BAR_TEMPTY + b));
-        if (!whole) {
-          ok = join(f, r.tile);
-          if (ok && share >= 0) {
-            int i = 0;
-            for (unsigned long long left = mask; left != 0; left &= left - 1, ++i) {
-              if (i % shares != share) continue;
-              const int m = __ffsll(static_cast<long long>(left)) - 1;
-              const float ga = total(f, r.tile, 0, m), up = total(f, r.tile, 1, m);
-              if (live) moe_store_h<T>(p, r.a, m, col, ga, up, vg, vu);
-            }
+        if (whole) continue;
+        ok = join(f, r.tile, slot);
+        if (!ok || share < 0) continue;
+        // This CTA's share of the tokens, a warp each; a lane has four columns.
+        const int col = col0 + 4 * lane;
+        const long long bi = static_cast<long long>(e) * p.H + col;
+        int i = 0;
+#pragma unroll 1
+        for (unsigned long long left = mask; left != 0; left &= left - 1, ++i) {
+          if (i % (4 * shares) != share * 4 + q) continue;
+          const int m = __ffsll(static_cast<long long>(left)) - 1;
+          const float4 ga = row_sum(m), up = row_sum(p.T + m);
+          if (col >= p.H) continue;
+          float v[4] = {ga.x, ga.y, ga.z, ga.w}, w[4] = {up.x, up.y, up.z, up.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[k] += moe_bias(bg, bi + k);
+            w[k] += moe_bias(bu, bi + k);
           }
+          act_values<false>(v, p.act);
+          __align__(8) T hi[4];
+          __align__(8) T lo[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) moe_split(v[k] * w[k], hi[k], lo[k]);
+          const long long at = (static_cast<long long>(r.a) * p.T + m) * p.H + col;
+          *reinterpret_cast<uint2*>(h_hi + at) = *reinterpret_cast<const uint2*>(hi);
+          *reinterpret_cast<uint2*>(h_lo + at) = *reinterpret_cast<const uint2*>(lo);
         }
       }
     }
@@ -703,9 +752,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
       for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
         const int b = local & 1;
         const int e = s_list[r.a];
-        const int col = r.tile * 256 + n;
-        const unsigned long long mask =
-            s_mask[2 * e] | (static_cast<unsigned long long>(s_mask[2 * e + 1]) << 32);
+        const unsigned long long mask = chosen_by(e);
         // The tokens' weights for this expert.
         float* const roww = s_roww + b * kMoeMaxT;
         if (et < p.T) {
@@ -715,11 +762,12 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
           roww[et] = w;
         }
         float vb[2] = {0.0f, 0.0f};
-        if (bo != nullptr && r.kb0 == 0) {
+        if (r.kb0 == 0) {  // (each expert's bias once a tile)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (col + 128 * h < p.D)
-              vb[h] = Tr::to_float(bo[static_cast<long long>(e) * p.D + col + 128 * h]);
+          for (int h = 0; h < 2; ++h) {
+            const int c = r.tile * 256 + 128 * h + n;
+            if (c < p.D) vb[h] = moe_bias(bo, static_cast<long long>(e) * p.D + c);
+          }
         }
         ok = named_bar_all(1, 128, mbar_wait(bar(S::BAR_TFULL + b),
                                              (static_cast<uint32_t>(local) >> 1) & 1u, abort_flag));
@@ -727,16 +775,17 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         tc_fence_after();
         const uint32_t acc = lane_addr + static_cast<uint32_t>(b * 2 * MN);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int mc = 0; mc < MN; mc += 16) {
+          const uint32_t some = static_cast<uint32_t>(mask >> mc) & 0xffffu;
+          if (some != 0) {
 #pragma unroll
-          for (int mc = 0; mc < MN; mc += 16) {
-            if (mc < p.T) {
+            for (int h = 0; h < 2; ++h) {
               uint32_t v[16];
               tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(h * MN + mc), v);
               tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 16; ++j)
-                if ((mask >> (mc + j)) & 1u)
+                if ((some >> j) & 1u)
                   y[h][mc + j] = fmaf(roww[mc + j], __uint_as_float(v[j]) + vb[h], y[h][mc + j]);
             }
           }
@@ -747,31 +796,32 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         // The CTA's last run of this tile?
         const int us = r.tile * f.per_tile, ue = us + f.per_tile;
         if (u + r.len < ue && u + r.len < f.u1) continue;
-        auto finish = [&](int h, int m, float sum) {
-          const int c = col + 128 * h;
-          if (c >= p.D) return;
-          if (res != nullptr) sum += Tr::to_float(res[m * p.ldr + c]);
-          Y[m * p.ldy + c] = Tr::from_float(sum);
-        };
-        const bool whole = f.u0 <= us && f.u1 >= ue;
         const int slot = f.u0 / f.per_tile == r.tile ? 0 : 1;
+        float* const to = part(g, slot) + n;
+        float* const to1 = to + p.T * 128;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int m = 0; m < MN; ++m) {
-            if (m < p.T) {
-              if (whole)
-                finish(h, m, y[h][m]);
-              else
-                part(g, slot, h, m)[n] = y[h][m];
-            }
-            y[h][m] = 0.0f;
+        for (int m = 0; m < MN; ++m) {
+          if (m < p.T) {
+            to[m * 128] = y[0][m];
+            to1[m * 128] = y[1][m];
           }
-        if (!whole) {
-          ok = join(f, r.tile);
-          if (ok && share >= 0)
-            for (int i = share; i < 2 * p.T; i += shares)
-              finish(i & 1, i >> 1, total(f, r.tile, i & 1, i >> 1));
+          y[0][m] = y[1][m] = 0.0f;
+        }
+        ok = join(f, r.tile, slot);
+        if (!ok || share < 0) continue;
+        // This CTA's share of the rows (halves of a token's 256 columns), a warp each.
+#pragma unroll 1
+        for (int row = share * 4 + q; row < 2 * p.T; row += 4 * shares) {
+          const float4 t = row_sum(row);
+          const int h = row >= p.T ? 1 : 0, m = row - h * p.T;
+          const int c = r.tile * 256 + 128 * h + 4 * lane;
+          if (c >= p.D) continue;
+          float v[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (res != nullptr) v[k] += Tr::to_float(res[m * p.ldr + c + k]);
+            Y[m * p.ldy + c + k] = Tr::from_float(v[k]);
+          }
         }
       }
     }
