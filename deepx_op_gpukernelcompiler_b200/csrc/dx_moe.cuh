@@ -13,8 +13,8 @@
 //     picks token i's experts.
 //   moe_experts_kernel  one CTA per SM, all resident (cooperative launch).
 //     Phase 1 computes h = act(gate) * up of every chosen expert, phase 2 the
-//     output; each phase's work units (tile x 64-deep K block) are dealt evenly
-//     and contiguously over the CTAs, so every SM streams the same bytes
+//     output; each phase's work is dealt evenly over the CTAs down to single
+//     64-deep K blocks of a tile (MoePhase), so every SM streams the same bytes
 //     whatever the sizes.  As in the skinny-M decode kernel the operands are
 //     swapped: 128 weight columns are the MMA's rows (an MN-major operand, as W
 //     lies in memory) and the tokens its columns.  All tokens go through every
@@ -250,19 +250,23 @@ struct MoeShape {
   }
 };
 
-// A run of K blocks that one accumulator collects: one tile's (phase 1), or one
-// tile's of one expert (phase 2).
+// A run of K blocks that one accumulator collects: of one tile (phase 1), or of
+// one tile and one expert (phase 2).
 struct MoeRun {
   int tile, a, kb0, len;  // a: index into the chosen experts
-  int u;                  // its first unit
 };
 
-// One phase's units and this CTA's share of them.
+// One phase's work of one CTA.  The `tiles - whole` tiles that do not make a full
+// wave of the grid are dealt out first, as units of one K block, evenly and
+// contiguously (a CTA gets parts of at most a few tiles); then come full waves of
+// whole tiles, whose epilogues need nobody else.  So the exchange of partial sums
+// runs beside the streaming of whole tiles, where a phase has any (phase 1 of
+// 8 tokens, 64 experts of 2048 x 1024: 336 tiles on 148 CTAs).
 struct MoePhase {
-  int units, ctas;  // CTAs that have units
-  int per_tile;     // units of a tile
-  int nt, kb;       // phase 1: tiles of an expert; K blocks of an expert's product
-  int u0, u1;
+  int tiles, whole, per_tile;  // tiles [0, whole) are whole; units of a tile
+  int units, ctas;             // of the split tiles; CTAs that have some
+  int nt, kb;                  // phase 1: tiles of an expert; K blocks of an expert's product
+  int u0, u1;                  // this CTA's units
   bool second;
 
   __device__ __forceinline__ int begin(int g) const {
@@ -273,10 +277,27 @@ struct MoePhase {
     while (g + 1 < ctas && begin(g + 1) <= u) ++g;
     return g;
   }
-  // The unit's tile, expert index and K block.
-  __device__ __forceinline__ void unit(int u, int& tile, int& a, int& kb_) const {
-    tile = u / per_tile;
-    const int r = u - tile * per_tile;
+  // The work item at position i of this CTA's list (its units, then the units of
+  // its whole tiles): tile, expert index and K block.
+  __device__ __forceinline__ int count() const {
+    const int mine = whole > static_cast<int>(blockIdx.x)
+                         ? (whole - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1
+                         : 0;
+    return u1 - u0 + mine * per_tile;
+  }
+  __device__ __forceinline__ void item(int i, int& tile, int& a, int& kb_) const {
+    int r;
+    if (i < u1 - u0) {
+      const int u = u0 + i;
+      tile = u / per_tile;
+      r = u - tile * per_tile;
+      tile += whole;
+    } else {
+      i -= u1 - u0;
+      const int w = i / per_tile;
+      r = i - w * per_tile;
+      tile = static_cast<int>(blockIdx.x) + w * static_cast<int>(gridDim.x);
+    }
     if (second) {
       a = r / kb;
       kb_ = r - a * kb;
@@ -285,24 +306,26 @@ struct MoePhase {
       kb_ = r;
     }
   }
-  __device__ __forceinline__ bool run(int u, MoeRun& r) const {
-    if (u >= u1) return false;
-    r.u = u;
-    unit(u, r.tile, r.a, r.kb0);
-    r.len = min(kb - r.kb0, u1 - u);
+  __device__ __forceinline__ bool run(int i, MoeRun& r) const {
+    if (i >= count()) return false;
+    item(i, r.tile, r.a, r.kb0);
+    r.len = kb - r.kb0;
+    if (i < u1 - u0) r.len = min(r.len, u1 - u0 - i);
     return true;
   }
 };
 
 __device__ __forceinline__ MoePhase moe_phase(const MoeParams& p, int chosen, bool second) {
   MoePhase f;
+  const int grid = static_cast<int>(gridDim.x), g = static_cast<int>(blockIdx.x);
   f.second = second;
   f.kb = second ? p.kb_h : p.kb_d;
   f.nt = p.nt_h;
   f.per_tile = second ? chosen * p.kb_h : p.kb_d;
-  f.units = second ? p.nt_d * f.per_tile : chosen * p.nt_h * f.per_tile;
-  f.ctas = min(static_cast<int>(gridDim.x), f.units);
-  const int g = static_cast<int>(blockIdx.x);
+  f.tiles = second ? p.nt_d : chosen * p.nt_h;
+  f.whole = f.tiles / grid * grid;
+  f.units = (f.tiles - f.whole) * f.per_tile;
+  f.ctas = min(grid, f.units);
   f.u0 = g < f.ctas ? f.begin(g) : 0;
   f.u1 = g < f.ctas ? f.begin(g + 1) : 0;
   return f;
@@ -437,70 +460,91 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
   if (warp == 0) {
     // ------------------------------------------------------ TMA producer
     if (lane == 0) {
+      // One thread feeds the SM, so it steps through runs and counts stages: with
+      // the divisions of MoePhase::item per unit it was what bound the kernel (8
+      // tokens, 64 experts: 122 us, 145 with two more divisions).
+      struct Cursor {
+        MoeRun r;
+        int at, i;  // the run's position in the phase, the block within the run
+        int stage;
+        uint32_t parity;
+      };
       const uint64_t pol = make_l2_policy_evict_first();
       const uint64_t keep = make_l2_policy_evict_last();
       uint32_t issued = 0;
       bool ok = true;
-      auto load_w = [&](int ph, int u, const MoePhase& f, int s) {
-        int tile, a, kb;
-        f.unit(u, tile, a, kb);
-        const int e = s_list[a];
-        const uint32_t fb = bar(S::BAR_FULL + s);
-        const uint32_t dst = sW + s * S::W_BYTES;
-        if (ph == 0) {
-          const int n = (tile - a * f.nt) * 128;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            tma_load_3d_hint(j < 2 ? &tmG : &tmU, dst + j * S::BOX_BYTES, fb, n + 64 * (j & 1),
-                             kb * S::BK, e, pol);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            tma_load_3d_hint(&tmO, dst + j * S::BOX_BYTES, fb, tile * 256 + 64 * j, kb * S::BK, e,
-                             pol);
+      Cursor w{}, t{};  // the next weights and the next tokens to load
+      auto seek = [](const MoePhase& f, Cursor& c) {
+        c.at = c.i = 0;
+        f.run(0, c.r);
+      };
+      auto advance = [stages](const MoePhase& f, Cursor& c) {
+        if (++c.stage == stages) {
+          c.stage = 0;
+          c.parity ^= 1u;
+        }
+        if (++c.i == c.r.len) {
+          c.at += c.r.len;
+          c.i = 0;
+          f.run(c.at, c.r);
         }
       };
-      auto load_t = [&](int ph, int u, const MoePhase& f, int s) {
-        int tile, a, kb;
-        f.unit(u, tile, a, kb);
+      // The stage of w.i, when it is free, with the weights on their way.
+      auto load_w = [&](const MoePhase& f, uint32_t bytes) {
+        const int s = w.stage;
+        if (!mbar_wait(bar(S::BAR_EMPTY + s), w.parity ^ 1u, abort_flag)) return false;
         const uint32_t fb = bar(S::BAR_FULL + s);
-        const uint32_t dst = sT + static_cast<uint32_t>(s) * 2 * t_bytes;
-        if (ph == 0) {
-          tma_load_2d_hint(&tmX, dst, fb, kb * S::BK, 0, keep);
+        mbar_arrive_expect_tx(fb, bytes);
+        const int e = s_list[w.r.a];
+        const int k = (w.r.kb0 + w.i) * S::BK;
+        const uint32_t dst = sW + s * S::W_BYTES;
+        if (!f.second) {
+          const int n = (w.r.tile - w.r.a * f.nt) * 128;
+          tma_load_3d_hint(&tmG, dst, fb, n, k, e, pol);
+          tma_load_3d_hint(&tmG, dst + S::BOX_BYTES, fb, n + 64, k, e, pol);
+          tma_load_3d_hint(&tmU, dst + 2 * S::BOX_BYTES, fb, n, k, e, pol);
+          tma_load_3d_hint(&tmU, dst + 3 * S::BOX_BYTES, fb, n + 64, k, e, pol);
         } else {
-          tma_load_2d_hint(&tmHi, dst, fb, kb * S::BK, a * p.T, keep);
-          tma_load_2d_hint(&tmLo, dst + t_bytes, fb, kb * S::BK, a * p.T, keep);
+          const int n = w.r.tile * 256;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tma_load_3d_hint(&tmO, dst + j * S::BOX_BYTES, fb, n + 64 * j, k, e, pol);
         }
+        advance(f, w);
+        ++issued;
+        return true;
+      };
+      auto load_t = [&](const MoePhase& f) {
+        const uint32_t fb = bar(S::BAR_FULL + t.stage);
+        const uint32_t dst = sT + static_cast<uint32_t>(t.stage) * 2 * t_bytes;
+        const int k = (t.r.kb0 + t.i) * S::BK;
+        if (!f.second) {
+          tma_load_2d_hint(&tmX, dst, fb, k, 0, keep);
+        } else {
+          tma_load_2d_hint(&tmHi, dst, fb, k, t.r.a * p.T, keep);
+          tma_load_2d_hint(&tmLo, dst + t_bytes, fb, k, t.r.a * p.T, keep);
+        }
+        advance(f, t);
       };
       for (int ph = 0; ok && ph < 2; ++ph) {
         const MoePhase f = moe_phase(p, chosen, ph != 0);
         const uint32_t bytes = S::W_BYTES + (ph != 0 ? 2 * t_bytes : t_bytes);
-        int u = f.u0;
-        auto start = [&](int unit) {  // the unit's stage, its weights on their way
-          const int s = static_cast<int>(issued % stages);
-          if (!mbar_wait(bar(S::BAR_EMPTY + s), ((issued / stages) & 1u) ^ 1u, abort_flag))
-            return false;
-          mbar_arrive_expect_tx(bar(S::BAR_FULL + s), bytes);
-          load_w(ph, unit, f, s);
-          ++issued;
-          return true;
-        };
+        const int items = f.count();
+        seek(f, w);
+        seek(f, t);
+        int u = 0;
         if (ph != 0) {
           // A ring of phase 2's weights before every h is written.
-          const uint32_t first = issued;
-          const int early = min(stages, f.u1 - f.u0);
-          int n = 0;
-          while (n < early && start(u + n)) ++n;
-          ok = n == early && moe_wait(barrier_ctr, static_cast<int>(gridDim.x), abort_flag);
+          const int early = min(stages, items);
+          while (u < early && load_w(f, bytes)) ++u;
+          ok = u == early && moe_wait(barrier_ctr, static_cast<int>(gridDim.x), abort_flag);
           fence_proxy_async_global();
           // (also when giving up, so that the started stages complete)
-          for (int i = 0; i < n; ++i)
-            load_t(ph, u + i, f, static_cast<int>((first + i) % stages));
-          u += n;
+          for (int i = 0; i < u; ++i) load_t(f);
         }
-        for (; ok && u < f.u1; ++u) {
-          ok = start(u);
-          if (ok) load_t(ph, u, f, static_cast<int>((issued - 1) % stages));
+        for (; ok && u < items; ++u) {
+          ok = load_w(f, bytes);
+          if (ok) load_t(f);
         }
       }
       // Loads in flight land before the shared memory is released.
@@ -519,7 +563,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
     for (int ph = 0; ok && ph < 2; ++ph) {
       const MoePhase f = moe_phase(p, chosen, ph != 0);
       MoeRun r;
-      for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
+      for (int u = 0; ok && f.run(u, r); u += r.len, ++local) {
         const int b = local & 1;
         if (!mbar_wait_warp(bar(S::BAR_TEMPTY + b), ((static_cast<uint32_t>(local) >> 1) & 1u) ^ 1u,
                             abort_flag)) {
@@ -594,21 +638,21 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
     // where the tile is its last one, waits until all are there.
     const float* sum = nullptr;
     int first = 0, peers = 1, share = 0, shares = 1;
-    auto join = [&](const MoePhase& f, int tile, int slot) {
-      const int us = tile * f.per_tile, ue = us + f.per_tile;
-      const bool whole = f.u0 <= us && f.u1 >= ue;
+    auto join = [&](const MoePhase& f, int tile, int slot, bool whole) {
       first = g;
       peers = shares = 1;
       share = 0;
       if (!whole) {
+        const int us = (tile - f.whole) * f.per_tile, ue = us + f.per_tile;
         first = f.cta_of(us);
         const int last = f.cta_of(ue - 1);
         peers = last - first + 1;
         shares = last - first + (f.begin(last + 1) == ue ? 1 : 0);
         share = f.u1 <= ue ? g - first : -1;
+        // (a CTA that starts inside the tile has it as its first tile)
+        if (first != g) slot = f.begin(first) / f.per_tile == tile - f.whole ? 0 : 1;
       }
-      // (a CTA that starts inside the tile has it as its first tile)
-      sum = part(first, first == g ? slot : (f.begin(first) / f.per_tile == tile ? 0 : 1));
+      sum = part(first, slot);
       __threadfence();
       named_bar_sync(1, 128);
       if (whole) return true;
@@ -648,13 +692,13 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
     {  // ---- phase 1: h
       const MoePhase f = moe_phase(p, chosen, false);
       MoeRun r;
-      for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
+      for (int u = 0; ok && f.run(u, r); u += r.len, ++local) {
         const int b = local & 1;
         const int e = s_list[r.a];
         const int col0 = (r.tile - r.a * f.nt) * 128;
         const unsigned long long mask = chosen_by(e);
         const bool whole = r.len == f.per_tile;
-        const int slot = f.u0 / f.per_tile == r.tile ? 0 : 1;
+        const int slot = f.u0 / f.per_tile + f.whole == r.tile ? 0 : 1;
         const bool live = col0 + n < p.H;
         float vg = 0.0f, vu = 0.0f;
         if (whole && live) {
@@ -704,7 +748,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(S::BAR_TEMPTY + b));
         if (whole) continue;
-        ok = join(f, r.tile, slot);
+        ok = join(f, r.tile, slot, false);
         if (!ok || share < 0) continue;
         // This CTA's share of the tokens, a warp each; a lane has four columns.
         const int col = col0 + 4 * lane;
@@ -749,7 +793,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
 #pragma unroll
         for (int m = 0; m < MN; ++m) y[h][m] = 0.0f;
       MoeRun r;
-      for (int u = f.u0; ok && f.run(u, r); u += r.len, ++local) {
+      for (int u = 0; ok && f.run(u, r); u += r.len, ++local) {
         const int b = local & 1;
         const int e = s_list[r.a];
         const unsigned long long mask = chosen_by(e);
@@ -793,10 +837,12 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(S::BAR_TEMPTY + b));
-        // The CTA's last run of this tile?
-        const int us = r.tile * f.per_tile, ue = us + f.per_tile;
-        if (u + r.len < ue && u + r.len < f.u1) continue;
-        const int slot = f.u0 / f.per_tile == r.tile ? 0 : 1;
+        // More of this tile to come?
+        MoeRun after;
+        if (f.run(u + r.len, after) && after.tile == r.tile) continue;
+        const int us = (r.tile - f.whole) * f.per_tile;
+        const bool whole = r.tile < f.whole || (f.u0 <= us && f.u1 >= us + f.per_tile);
+        const int slot = r.tile >= f.whole && f.u0 / f.per_tile + f.whole == r.tile ? 0 : 1;
         float* const to = part(g, slot) + n;
         float* const to1 = to + p.T * 128;
 #pragma unroll
@@ -807,7 +853,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
           }
           y[0][m] = y[1][m] = 0.0f;
         }
-        ok = join(f, r.tile, slot);
+        ok = join(f, r.tile, slot, whole);
         if (!ok || share < 0) continue;
         // This CTA's share of the rows (halves of a token's 256 columns), a warp each.
 #pragma unroll 1

@@ -142,11 +142,11 @@ int launch_moe_experts(const dx_moe_args& a, int dev, int ctas, const MoeLayout&
   set_plan("moe T=%d mn=%d stages=%d grid=%d smem=%d workspace=%zu", p.T, mn, stages, ctas, smem,
            l.bytes);
   // Cooperative: the CTAs wait for one another, so all of them or none are placed.
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeCooperative;
-  attr[0].val.cooperative = 1;
-  cudaLaunchConfig_t cfg = launch_config(ctas, S::THREADS, smem, stream, 1, attr, false);
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[3];
+  cudaLaunchConfig_t cfg = launch_config(ctas, S::THREADS, smem, stream, 1, attr);
+  attr[cfg.numAttrs].id = cudaLaunchAttributeCooperative;
+  attr[cfg.numAttrs].val.cooperative = 1;
+  ++cfg.numAttrs;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tG, tU, tO, tX, tHi, tLo, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch moe_experts_kernel");
