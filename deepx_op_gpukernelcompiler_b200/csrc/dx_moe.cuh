@@ -43,9 +43,9 @@ constexpr int kMoeMaxE = 256;
 constexpr int kMoeMaxTop = 32;
 
 // ---------------------------------------------------------------- router
-constexpr int kRouterThreads = 512;
+constexpr int kRouterThreads = 1024;
 constexpr int kRouterTokens = 8;  // tokens of a cluster = its CTAs
-constexpr int kRouterRows = 256;  // rows of Wr per step
+constexpr int kRouterRows = 512;  // rows of Wr per step, at most
 
 struct MoeRouterParams {
   const void* X;
@@ -68,8 +68,9 @@ __device__ __forceinline__ uint32_t moe_key(float f) {
 template <typename T>
 __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRouterParams p) {
   using Tr = ElemTraits<T>;
-  __shared__ __align__(16) float s_x[kRouterRows][kRouterTokens];
-  __shared__ float s_part[kRouterThreads * kRouterTokens];  // [row group][token][expert]
+  __shared__ __align__(16) float s_x[kRouterThreads][kRouterTokens];  // [row][token]
+  static_assert(kRouterRows <= kRouterThreads, "a step's rows");
+  float* const s_part = &s_x[0][0];  // [row group][token][expert], once s_x is done with
   __shared__ float s_sum[kRouterTokens][kMoeMaxE];
   __shared__ float s_logit[kMoeMaxE];
   const int tid = static_cast<int>(threadIdx.x);
@@ -81,7 +82,8 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRou
   if (blockIdx.x == 0)
     for (int i = tid; i < p.num_counters; i += kRouterThreads) p.counters[i] = 0;
 
-  // Threads as row groups x experts; each sums its rows for all tokens.
+  // Threads as row groups x experts; each sums its rows for all tokens.  Wr's rows
+  // are asked for before the tokens' values are needed: one trip to memory a step.
   const int ep = (p.E + 31) / 32 * 32;
   const int groups = kRouterThreads / ep;
   const int e = tid % ep, kg = tid / ep;
@@ -90,45 +92,53 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRou
   const int k_begin = rank * slice, k_end = min(p.D, k_begin + slice);
   const T* const X = static_cast<const T*>(p.X);
   const T* const Wr = static_cast<const T*>(p.Wr);
+  constexpr int kBatch = 16;                                            // rows of Wr a thread, per step
+  constexpr int kPerThread = kRouterRows * kRouterTokens / kRouterThreads;  // token values
+  const int step = min(kRouterRows, kBatch * groups);  // rows of Wr per step
   float acc[kRouterTokens];
 #pragma unroll
   for (int t = 0; t < kRouterTokens; ++t) acc[t] = 0.0f;
-  for (int k0 = k_begin; k0 < k_end; k0 += kRouterRows) {
-    const int rows = min(kRouterRows, k_end - k0);
-    __syncthreads();
-    for (int i = tid; i < kRouterRows * kRouterTokens; i += kRouterThreads) {
-      const int t = i / kRouterRows, k = i % kRouterRows;
-      s_x[k][t] = t < tokens && k < rows ? Tr::to_float(X[(t0 + t) * p.ldx + k0 + k]) : 0.0f;
+  for (int k0 = k_begin; k0 < k_end; k0 += step) {
+    const int rows = min(step, k_end - k0);
+    T w[kBatch], x[kPerThread];
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const int at = i * kRouterThreads + tid, t = at / kRouterRows, k = at % kRouterRows;
+      x[i] = t < tokens && k < rows ? X[(t0 + t) * p.ldx + k0 + k] : Tr::from_float(0.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int k = kg + i * groups;
+      w[i] = live && k < rows ? Wr[(k0 + k) * p.ldwr + e] : Tr::from_float(0.0f);
+    }
+    if (k0 != k_begin) __syncthreads();  // the previous step's values are no longer read
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const int at = i * kRouterThreads + tid;
+      s_x[at % kRouterRows][at / kRouterRows] = Tr::to_float(x[i]);
     }
     __syncthreads();
     if (live) {
-      constexpr int kBatch = 16;  // rows whose loads are issued together
-      for (int k = kg; k < rows; k += kBatch * groups) {
-        float w[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int kk = k + i * groups;
-          w[i] = kk < rows ? Tr::to_float(Wr[(k0 + kk) * p.ldwr + e]) : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int kk = k + i * groups;
-          if (kk < rows) {
-            const float4 a = *reinterpret_cast<const float4*>(&s_x[kk][0]);
-            const float4 b = *reinterpret_cast<const float4*>(&s_x[kk][4]);
-            acc[0] = fmaf(a.x, w[i], acc[0]);
-            acc[1] = fmaf(a.y, w[i], acc[1]);
-            acc[2] = fmaf(a.z, w[i], acc[2]);
-            acc[3] = fmaf(a.w, w[i], acc[3]);
-            acc[4] = fmaf(b.x, w[i], acc[4]);
-            acc[5] = fmaf(b.y, w[i], acc[5]);
-            acc[6] = fmaf(b.z, w[i], acc[6]);
-            acc[7] = fmaf(b.w, w[i], acc[7]);
-          }
+      for (int i = 0; i < kBatch; ++i) {
+        const int k = kg + i * groups;
+        if (k < rows) {
+          const float f = Tr::to_float(w[i]);
+          const float4 a = *reinterpret_cast<const float4*>(&s_x[k][0]);
+          const float4 b = *reinterpret_cast<const float4*>(&s_x[k][4]);
+          acc[0] = fmaf(a.x, f, acc[0]);
+          acc[1] = fmaf(a.y, f, acc[1]);
+          acc[2] = fmaf(a.z, f, acc[2]);
+          acc[3] = fmaf(a.w, f, acc[3]);
+          acc[4] = fmaf(b.x, f, acc[4]);
+          acc[5] = fmaf(b.y, f, acc[5]);
+          acc[6] = fmaf(b.z, f, acc[6]);
+          acc[7] = fmaf(b.w, f, acc[7]);
         }
       }
     }
   }
+  __syncthreads();
   if (kg < groups) {
 #pragma unroll
     for (int t = 0; t < kRouterTokens; ++t) s_part[(kg * kRouterTokens + t) * ep + e] = acc[t];
