@@ -63,12 +63,13 @@ def quantize_rows(X: torch.Tensor) -> Int8Rows:
     _check_matrix("X", X, None, None)
     M, K = X.shape
     q = _empty_rows(M, K, X.device)
-    scale = torch.empty((M,), dtype=torch.float32, device=X.device)
-    with torch.cuda.device(X.device):
-        rc = nat.load().dx_quantize_rows(
-            X.data_ptr(), q.data_ptr(), scale.data_ptr(), M, K, _ld(X), max(q.stride(0), K),
-            DTYPE_CODES[X.dtype], torch.cuda.current_stream(X.device).cuda_stream)
-    nat.check("dx_quantize_rows", rc)
+    scale = X.new_empty(M, dtype=torch.float32)
+    lib = nat.load()
+    rc = _on_device(X.get_device(), lambda stream: lib.dx_quantize_rows(
+        X.data_ptr(), q.data_ptr(), scale.data_ptr(), M, K, _ld(X), max(q.stride(0), K),
+        DTYPE_CODES[X.dtype], stream))
+    if rc:
+        nat.check("dx_quantize_rows", rc)
     return Int8Rows(q, scale)
 
 
@@ -94,6 +95,11 @@ def int8_rows(q: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
     return Int8Rows(q, scale.contiguous())
 
 
+# The current stream's handle without building a Stream object (2 us a call).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def _pair(name: str, rows, K: int | None, n: int | None) -> tuple:
     """Checks an (int8 rows, scales) pair -> (q, scale, rows, K, pitch)."""
     if not isinstance(rows, tuple) or len(rows) != 2:
@@ -102,14 +108,17 @@ def _pair(name: str, rows, K: int | None, n: int | None) -> tuple:
     if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise ValueError(f"{name} must hold int8 rows and float32 scales, got {q.dtype} and "
                          f"{scale.dtype}")
-    if q.dim() != 2:
-        raise ValueError(f"{name} must be 2-D, got shape {tuple(q.shape)}")
-    rows_, cols = q.shape
+    shape = q.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} must be 2-D, got shape {tuple(shape)}")
+    rows_, cols = shape
     ld, unit = q.stride()
-    if (K is not None and cols != K) or (n is not None and rows_ != n) or unit != 1 or ld < cols:
+    if unit != 1 or ld < cols or (K is not None and cols != K) or (n is not None and rows_ != n):
         _check_matrix(name, q, n, K)  # raises, unless the stride of a lone row or column is odd
-    if scale.dim() != 1 or scale.shape[0] != rows_ or not scale.is_contiguous():
+    if scale.shape != (rows_,) or (rows_ > 1 and scale.stride(0) != 1):
         raise ValueError(f"{name} needs one contiguous scale per row, got {tuple(scale.shape)}")
+    if scale.get_device() != q.get_device():
+        raise ValueError(f"{name}'s scales are on {scale.device}, its rows on {q.device}")
     if rows_ <= 1:
         ld = -(-cols // 16) * 16
     if ld % 16 or q.data_ptr() % 16:
@@ -121,22 +130,33 @@ def _pair(name: str, rows, K: int | None, n: int | None) -> tuple:
 def _float_or_pair(X, dtype):
     """X of a product -> (x, dtype code, scale, M, K, pitch, output dtype)."""
     if isinstance(X, torch.Tensor):
-        code = DTYPE_CODES.get(X.dtype)
+        x_dtype = X.dtype
+        code = DTYPE_CODES.get(x_dtype)
         if code is None:
-            raise ValueError(f"unsupported dtype {X.dtype}; expected float32, float16 or "
+            raise ValueError(f"unsupported dtype {x_dtype}; expected float32, float16 or "
                              f"bfloat16, or a pair (int8 rows, scales)")
-        _check_matrix("X", X, None, None)
-        M, K = X.shape
-        x, scale, ld, out_dtype = X, None, _ld(X), X.dtype if dtype is None else dtype
+        shape = X.shape
+        if len(shape) != 2:
+            raise ValueError(f"X must be 2-D, got shape {tuple(shape)}")
+        M, K = shape
+        ld, unit = X.stride()
+        if unit != 1 or ld < K:
+            _check_matrix("X", X, None, None)
+            ld = _ld(X)
+        x, scale = X, None
+        if dtype is None:
+            dtype = x_dtype
     else:
         x, scale, M, K, ld = _pair("X", X, None, None)
-        code, out_dtype = nat.DX_DTYPE_I8, torch.bfloat16 if dtype is None else dtype
-    if out_dtype not in DTYPE_CODES:
-        raise ValueError(f"unsupported output dtype {out_dtype}; expected float32, float16 or "
+        code = nat.DX_DTYPE_I8
+        if dtype is None:
+            dtype = torch.bfloat16
+    if dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported output dtype {dtype}; expected float32, float16 or "
                          f"bfloat16")
     if K < 1:
         raise ValueError("X must have at least one column")
-    return x, code, scale, M, K, ld, out_dtype
+    return x, code, scale, M, K, ld, dtype
 
 
 def _kernel(kernel: str) -> int:
@@ -146,18 +166,25 @@ def _kernel(kernel: str) -> int:
     return code
 
 
-def _output(name: str, out, x: torch.Tensor, M: int, N: int, dtype: torch.dtype) -> torch.Tensor:
-    if x.device.type != "cuda":
+def _same_device(x: torch.Tensor, index: int, *named) -> None:
+    for name, t in named:
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, X is on {x.device}")
+
+
+def _output(name: str, out, x: torch.Tensor, M: int, N: int, dtype: torch.dtype):
+    """-> (Y, its pitch)."""
+    if not x.is_cuda:
         raise ValueError(f"{name} runs on CUDA tensors only (the engine has no CPU path)")
     if out is None:
-        return torch.empty((M, N), dtype=dtype, device=x.device)
+        return x.new_empty((M, N), dtype=dtype), max(N, 1)
     _check_matrix("out", out, M, N)
     _like("out", out, x, dtype)
-    return out
+    return out, _ld(out)
 
 
-def _like(name: str, t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype | None) -> None:
-    if dtype is not None and t.dtype is not dtype:
+def _like(name: str, t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype) -> None:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} dtype {t.dtype} differs from the output dtype {dtype}")
     if t.get_device() != x.get_device():
         raise ValueError(f"{name} is on {t.device}, X is on {x.device}")
@@ -167,33 +194,18 @@ def _vector(name: str, b: torch.Tensor | None, N: int, x: torch.Tensor, dtype: t
     """Checks a bias -> its address (None without one)."""
     if b is None:
         return None
-    if b.dim() != 1 or b.shape[0] != N or not b.is_contiguous():
+    if b.shape != (N,) or not b.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of shape ({N},)")
     _like(name, b, x, dtype)
     return b.data_ptr()
 
 
-class _on:
-    """The device of x made current for a launch; `stream` is its current stream's handle."""
-
-    __slots__ = ("guard", "stream")
-
-    def __init__(self, x: torch.Tensor):
-        index = x.get_device()
-        self.guard = None
-        if index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(index)
-        self.stream = torch.cuda.current_stream(index).cuda_stream
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _on_device(index: int, call):
+    """call(stream) with device `index` current; `stream` is its current stream's handle."""
+    if index == _current_device():
+        return call(_raw_stream(index))
+    with torch.cuda.device(index):
+        return call(_raw_stream(index))
 
 
 def _workspace(lib, x: torch.Tensor, x_scale, M: int, K: int):
@@ -202,8 +214,9 @@ def _workspace(lib, x: torch.Tensor, x_scale, M: int, K: int):
     # it, and the allocator keeps it from others until the launches are done.
     if x_scale is not None or M == 0:
         return None, None, 0
-    space = torch.empty(lib.dx_int8_workspace_size(M, K), dtype=torch.uint8, device=x.device)
-    return space, space.data_ptr(), space.numel()
+    size = lib.dx_int8_workspace_size(M, K)
+    space = x.new_empty(size, dtype=torch.uint8)
+    return space, space.data_ptr(), size
 
 
 def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
@@ -218,10 +231,9 @@ def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
     act, kcode = activation_code(activation), _kernel(kernel)
     x, x_code, x_scale, M, K, ldx, dtype = _float_or_pair(X, dtype)
     wq, ws, N, _, ldw = _pair("W", W, K, None)
-    out = _output("int8_linear", out, x, M, N, dtype)
-    for name, t in (("W", wq), ("W's scale", ws), ("X's scale", x_scale)):
-        if t is not None:
-            _like(name, t, x, None)
+    out, ldy = _output("int8_linear", out, x, M, N, dtype)
+    index = x.get_device()
+    _same_device(x, index, ("W", wq))
     b_ptr = _vector("bias", bias, N, x, dtype)
     r_ptr, ldr = None, 0
     if residual is not None:
@@ -229,12 +241,15 @@ def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
         _like("residual", residual, x, dtype)
         r_ptr, ldr = residual.data_ptr(), _ld(residual)
     lib = nat.load()
-    with _on(x) as stream:
+
+    def call(stream):
         space, ws_ptr, ws_bytes = _workspace(lib, x, x_scale, M, K)
-        rc = lib.dx_int8_linear(
+        return lib.dx_int8_linear(
             x.data_ptr(), x_code, x_scale.data_ptr() if x_scale is not None else None,
             wq.data_ptr(), ws.data_ptr(), b_ptr, r_ptr, out.data_ptr(), M, N, K, ldx, ldw, ldr,
-            _ld(out), DTYPE_CODES[dtype], act, kcode, ws_ptr, ws_bytes, stream)
+            ldy, DTYPE_CODES[dtype], act, kcode, ws_ptr, ws_bytes, stream)
+
+    rc = _on_device(index, call)
     if rc:
         nat.check("dx_int8_linear", rc)
     return out
@@ -250,21 +265,22 @@ def int8_gated_linear(X, Wg, Wu, bias_g: torch.Tensor | None = None,
     x, x_code, x_scale, M, K, ldx, dtype = _float_or_pair(X, dtype)
     gq, gs, N, _, ldg = _pair("Wg", Wg, K, None)
     uq, us, _, _, ldu = _pair("Wu", Wu, K, N)
-    out = _output("int8_gated_linear", out, x, M, N, dtype)
-    for name, t in (("Wg", gq), ("Wg's scale", gs), ("Wu", uq), ("Wu's scale", us),
-                    ("X's scale", x_scale)):
-        if t is not None:
-            _like(name, t, x, None)
+    out, ldy = _output("int8_gated_linear", out, x, M, N, dtype)
+    index = x.get_device()
+    _same_device(x, index, ("Wg", gq), ("Wu", uq))
     bg_ptr = _vector("bias_g", bias_g, N, x, dtype)
     bu_ptr = _vector("bias_u", bias_u, N, x, dtype)
     lib = nat.load()
-    with _on(x) as stream:
+
+    def call(stream):
         space, ws_ptr, ws_bytes = _workspace(lib, x, x_scale, M, K)
-        rc = lib.dx_int8_gated_linear(
+        return lib.dx_int8_gated_linear(
             x.data_ptr(), x_code, x_scale.data_ptr() if x_scale is not None else None,
             gq.data_ptr(), gs.data_ptr(), uq.data_ptr(), us.data_ptr(), bg_ptr, bu_ptr,
-            out.data_ptr(), M, N, K, ldx, ldg, ldu, _ld(out), DTYPE_CODES[dtype], act, kcode,
-            ws_ptr, ws_bytes, stream)
+            out.data_ptr(), M, N, K, ldx, ldg, ldu, ldy, DTYPE_CODES[dtype], act, kcode, ws_ptr,
+            ws_bytes, stream)
+
+    rc = _on_device(index, call)
     if rc:
         nat.check("dx_int8_gated_linear", rc)
     return out

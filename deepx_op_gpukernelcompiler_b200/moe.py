@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from . import _native as nat
-from .int8 import _like, _on
+from .int8 import _like, _on_device
 from .linear import DTYPE_CODES, _check_matrix, _ld, activation_code
 
 MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 256, 32
@@ -90,27 +90,30 @@ def moe_ffn(X: torch.Tensor, Wr: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tenso
     if X.device.type != "cuda":
         raise ValueError("moe_ffn runs on CUDA tensors only (the engine has no CPU path)")
     if out is None:
-        out = torch.empty((T, D), dtype=X.dtype, device=X.device)
+        out = X.new_empty((T, D))
     else:
         _check_matrix("out", out, T, D)
         _like("out", out, X, X.dtype)
     if X.data_ptr() % 16 or (T > 1 and X.stride(0) % 8):
         X = X.contiguous() if not X.is_contiguous() else X.clone()
-    routing = torch.empty((2, T, top_k), dtype=torch.float32, device=X.device)
+    routing = X.new_empty((2, T, top_k), dtype=torch.float32)
     weights, ids = routing[0], routing[1].view(torch.int32)
     lib = nat.load()
-    with _on(X) as stream:
+
+    def call(stream):
         # Of this call alone, from the allocator of the current stream or of the
         # graph being captured.
-        space = torch.empty(lib.dx_moe_workspace_size(T, H, E, top_k), dtype=torch.uint8,
-                            device=X.device)
+        size = lib.dx_moe_workspace_size(T, H, E, top_k)
+        space = X.new_empty(size, dtype=torch.uint8)
         args = nat.MoeArgs(
             X.data_ptr(), Wr.data_ptr(), br_ptr, Wg.data_ptr(), Wu.data_ptr(), Wo.data_ptr(),
             bg_ptr, bu_ptr, bo_ptr, r_ptr, out.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, D,
             H, E, top_k, _ld(X), _ld(Wr), Wg.stride(1), Wg.stride(0), Wu.stride(1), Wu.stride(0),
             Wo.stride(1), Wo.stride(0), ldr, _ld(out), code, act, 1 if renormalize else 0,
-            space.data_ptr(), space.numel())
-        rc = lib.dx_moe(ctypes.addressof(args), stream)
+            space.data_ptr(), size)
+        return lib.dx_moe(ctypes.addressof(args), stream)
+
+    rc = _on_device(X.get_device(), call)
     if rc:
         nat.check("dx_moe", rc)
     return (out, weights, ids) if return_routing else out
