@@ -41,13 +41,16 @@ struct Int8Params {
   void* Y;
   int act;
   // tile kernel
+  int nr;       // channels of a tile: up to 128 (gated: 64), a multiple of 8
   int mn;       // tokens of a tile: a multiple of 16 up to 128
   int cluster;  // CTAs that split K
   int w_early;  // the preceding launch wrote only X: W may be read before it ends
   int stages;   // of the operand ring (both kernels)
   // pair kernel
   int bn;       // accumulator columns of a tile: a multiple of 32 (gated: 64) up to 256
-  int m_tiles, num_tiles, n_tiles, group_m, workers;
+  int m_tiles, n_tiles, group_m, workers;
+  int full_tiles;  // tiles [full_tiles, m_tiles * n_tiles) are done as two halves each
+  int num_work;    // full_tiles + 2 * the others
   int has_residual;
 };
 
@@ -102,7 +105,6 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
                      const __grid_constant__ CUtensorMap tmX, const Int8Params p) {
   using S = Int8TileShape;
   using Tr = ElemTraits<T>;
-  constexpr int NT = kGated ? 64 : 128;  // output channels of the tile
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base = (raw_u32 + 1023u) & ~1023u;
@@ -110,6 +112,9 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
   const int stages = p.stages;
   const uint32_t x_bytes = static_cast<uint32_t>(p.mn) * S::BK;
   const uint32_t stage_bytes = S::W_BYTES + x_bytes;
+  // What a stage loads: with fewer than 128 rows the MMA reads stale rows behind
+  // them, whose results nobody uses.
+  const uint32_t load_bytes = static_cast<uint32_t>(p.nr * (kGated ? 2 : 1)) * S::BK + x_bytes;
   const uint32_t sW = base;
   const uint32_t sX = base + static_cast<uint32_t>(stages) * S::W_BYTES;
   const uint32_t tail = static_cast<uint32_t>(stages) * stage_bytes;
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
   const int lane = threadIdx.x & 31;
   const int C = p.cluster;
   const int c = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int n0 = static_cast<int>(blockIdx.x) / C * NT;
+  const int n0 = static_cast<int>(blockIdx.x) / C * p.nr;
   const int m0 = static_cast<int>(blockIdx.y) * p.mn;
   const int rows = min(p.mn, p.M - m0);
   const int kb0 = static_cast<int>(static_cast<long long>(c) * p.k_blocks / C);
@@ -169,7 +174,7 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
   const int early = min(stages, kb1 - kb0);
   if (producer && p.w_early) {
     for (int i = 0; i < early; ++i) {
-      mbar_arrive_expect_tx(bar(S::BAR_FULL + i), stage_bytes);
+      mbar_arrive_expect_tx(bar(S::BAR_FULL + i), load_bytes);
       load_w(i, kb0 + i, bar(S::BAR_FULL + i), pol_w);
     }
   }
@@ -184,7 +189,8 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
   bool done = true;  // epilogue: the accumulator is complete
   // The channel this epilogue thread finishes, and its scales and biases.
   const bool via_smem = kGated || C > 1;
-  const int ncol = n0 + (kGated ? (et & 63) : (via_smem ? et : q * 32 + lane));
+  const int nt = kGated ? (et & 63) : (via_smem ? et : q * 32 + lane);
+  const int ncol = nt < p.nr ? n0 + nt : p.N;  // (p.N: none)
   float t0 = 0.0f, t1 = 0.0f, b0 = 0.0f, b1 = 0.0f;
 
   if (warp == 0) {
@@ -196,7 +202,7 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
         const uint32_t fb = bar(S::BAR_FULL + s);
         if (!(p.w_early && i < early)) {
           if (!mbar_wait(bar(S::BAR_EMPTY + s), ph ^ 1u, abort_flag)) break;
-          mbar_arrive_expect_tx(fb, stage_bytes);
+          mbar_arrive_expect_tx(fb, load_bytes);
           load_w(s, kb, fb, pol_w);
         }
         tma_load_2d(&tmX, sX + s * x_bytes, fb, kb * S::BK, m0);
@@ -379,7 +385,28 @@ struct Int8PairShape {
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
 
-// The tile'th tile: m-tiles fastest inside groups of group_m (as umma_tile_coords).
+// A pair's piece of work: a tile, or half the columns of one.
+struct Int8Work {
+  int mb, nb, half, bn;  // bn: accumulator columns (the tile's, or half of them)
+};
+
+__device__ __forceinline__ void int8_tile_coords(const Int8Params& p, int t, int& mb, int& nb);
+
+__device__ __forceinline__ Int8Work int8_work(const Int8Params& p, int i) {
+  Int8Work w;
+  w.half = 0;
+  w.bn = p.bn;
+  int t = i;
+  if (i >= p.full_tiles) {
+    t = p.full_tiles + ((i - p.full_tiles) >> 1);
+    w.half = (i - p.full_tiles) & 1;
+    w.bn = p.bn / 2;
+  }
+  int8_tile_coords(p, t, w.mb, w.nb);
+  return w;
+}
+
+// The t'th tile: m-tiles fastest inside groups of group_m (as umma_tile_coords).
 __device__ __forceinline__ void int8_tile_coords(const Int8Params& p, int t, int& mb, int& nb) {
   const int per_group = p.group_m * p.n_tiles;
   const int g = t / per_group;
@@ -425,8 +452,8 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base = (raw_u32 + 1023u) & ~1023u;
   uint8_t* const base_ptr = smem_raw + (base - raw_u32);
-  const int bn_cta = p.bn / 2;  // W rows staged by each CTA
-  const uint32_t b_bytes = static_cast<uint32_t>(bn_cta) * S::BK;
+  const uint32_t b_bytes = static_cast<uint32_t>(p.bn / 2) * S::BK;  // a stage's W rows, per CTA
+  const int box_rows = p.bn / 4;                                     // per load
   const uint32_t sA = base;
   const uint32_t sB = base + static_cast<uint32_t>(p.stages) * S::A_BYTES;
   const uint32_t bars = base + S::OFF_BAR;
@@ -479,21 +506,28 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
       int s = 0;
       uint32_t ph = 0, issued = 0;
       bool ok = true;
-      for (int tile = pair; ok && tile < p.num_tiles; tile += p.workers) {
-        int mb, nb;
-        int8_tile_coords(p, tile, mb, nb);
-        const int m0 = mb * 2 * S::BM + static_cast<int>(rank) * S::BM;
-        const int n0 = kGated ? nb * bn_cta : nb * p.bn + static_cast<int>(rank) * bn_cta;
+      for (int i = pair; ok && i < p.num_work; i += p.workers) {
+        const Int8Work wk = int8_work(p, i);
+        const int m0 = wk.mb * 2 * S::BM + static_cast<int>(rank) * S::BM;
+        // Plain: a tile's columns are the leader's, then the peer's; gated: both
+        // CTAs load the same columns, the leader of Wg and the peer of Wu.
+        const int n0 = kGated ? wk.nb * (p.bn / 2) + wk.half * box_rows
+                              : wk.nb * p.bn + wk.half * wk.bn + static_cast<int>(rank) * (wk.bn / 2);
+        const bool wide = wk.bn == p.bn;
+        const uint32_t bytes = 2 * (S::A_BYTES + static_cast<uint32_t>(wk.bn / 2) * S::BK);
         const CUtensorMap* const mapB = (kGated && rank != 0) ? &tmB2 : &tmB;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!mbar_wait(bar(S::BAR_EMPTY + s), ph ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          if (leader) mbar_arrive_expect_tx(bar(S::BAR_FULL + s), 2 * (S::A_BYTES + b_bytes));
+          if (leader) mbar_arrive_expect_tx(bar(S::BAR_FULL + s), bytes);
           const uint32_t fb = mapa_shared(bar(S::BAR_FULL + s), 0);
           tma_load_2d_pair(&tmA, sA + s * S::A_BYTES, fb, kb * S::BK, m0, pol);
           tma_load_2d_pair(mapB, sB + s * b_bytes, fb, kb * S::BK, n0, pol);
+          if (wide)
+            tma_load_2d_pair(mapB, sB + s * b_bytes + b_bytes / 2, fb, kb * S::BK, n0 + box_rows,
+                             pol);
           ++issued;
           if (++s == p.stages) {
             s = 0;
@@ -512,12 +546,12 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
   } else if (warp == 1) {
     // ----------------------------------------------- MMA issuer (leader)
     if (leader) {
-      const uint32_t idesc = umma_idesc_i8(256, p.bn);
       const bool issuer = elect_one();
       int s = 0, local = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int tile = pair; ok && tile < p.num_tiles; tile += p.workers, ++local) {
+      for (int i = pair; ok && i < p.num_work; i += p.workers, ++local) {
+        const uint32_t idesc = umma_idesc_i8(256, i < p.full_tiles ? p.bn : p.bn / 2);
         const int b = local & 1;
         const uint32_t use_ph = (static_cast<uint32_t>(local) >> 1) & 1u;
         if (!mbar_wait_warp(bar(S::BAR_TEMPTY + b), use_ph ^ 1u, abort_flag)) break;
@@ -554,11 +588,6 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
     // --------------------------------------------- epilogue (both CTAs)
     const int e = warp - 2;
     const int q = warp & 3;
-    // Output columns of a tile, and this warp's half of their 32-column chunks.
-    const int out_cols = kGated ? bn_cta : p.bn;
-    const int half = (out_cols / 32 + 1) / 2;
-    const int c0 = (e / 4) * half * 32;
-    const int chunks = e / 4 == 0 ? half : out_cols / 32 - half;
     EpilogueCtx<T> c;
     c.tmY = &tmY;
     c.tmR = &tmR;
@@ -573,13 +602,17 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
     float* const vec = reinterpret_cast<float*>(base_ptr + S::OFF_VEC + e * S::VEC_BYTES);
     uint32_t it = 0;
     int local = 0;
-    for (int tile = pair; tile < p.num_tiles; tile += p.workers, ++local) {
+    for (int i = pair; i < p.num_work; i += p.workers, ++local) {
       const int b = local & 1;
       const uint32_t use_ph = (static_cast<uint32_t>(local) >> 1) & 1u;
-      int mb, nb;
-      int8_tile_coords(p, tile, mb, nb);
-      const int n0 = nb * out_cols + c0;
-      const int row_base = mb * 2 * S::BM + static_cast<int>(rank) * S::BM + q * 32;
+      const Int8Work wk = int8_work(p, i);
+      // Output columns of the work, and this warp's half of their 32-column chunks.
+      const int out_cols = kGated ? wk.bn / 2 : wk.bn;
+      const int half = (out_cols / 32 + 1) / 2;
+      const int c0 = (e / 4) * half * 32;
+      const int chunks = e / 4 == 0 ? half : out_cols / 32 - half;
+      const int n0 = wk.nb * (kGated ? p.bn / 2 : p.bn) + wk.half * out_cols + c0;
+      const int row_base = wk.mb * 2 * S::BM + static_cast<int>(rank) * S::BM + q * 32;
       const int row = row_base + lane;
       const float sx = row < p.M ? p.sx[row] : 0.0f;
       __syncwarp();  // the previous tile's values are no longer read
@@ -612,7 +645,7 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
       // (the first chunk's residual was asked for before the accumulator was ready)
       uint32_t r[32], u[32];
       tmem_ld_32x32b_x32(acc, r);
-      if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(bn_cta), u);
+      if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(wk.bn / 2), u);
       bool ok = true;
 #pragma unroll 1
       for (int ch = 0; ch < live; ++ch) {
@@ -624,7 +657,7 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
         if (kGated) int8_scale(w, u, sx, vec + 256 + 32 * ch, vec + 384 + 32 * ch);
         if (ch + 1 < live) {
           tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(32 * (ch + 1)), r);
-          if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(bn_cta + 32 * (ch + 1)), u);
+          if (kGated) tmem_ld_32x32b_x32(acc + static_cast<uint32_t>(wk.bn / 2 + 32 * (ch + 1)), u);
         } else {
           tc_fence_before();
           __syncwarp();

@@ -152,8 +152,9 @@ bool int8_pair_eligible(const Int8Problem& p) {
 struct Int8Plan {
   bool pair = false;
   int bn = 256;               // pair
+  bool halves = false;        // pair: the last wave's tiles as two halves each
   int workers = 0;            // pair
-  int mn = 16, cluster = 1, stages = 3;  // tile
+  int nr = 128, mn = 16, cluster = 1, stages = 3;  // tile
 };
 
 // Tile kernel: tokens per tile, CTAs per cluster and ring depth (B200; us, W in
@@ -167,22 +168,37 @@ struct Int8Plan {
 //   for 1; K = 14336: 11.3 for 7, 14.5 for 3; K = N = 1024: 4.0 for 4, 5.3 for 1.
 //   Beyond a wave it only costs: M = 16, N = 28672: 41 for 1, 45 for 2.
 //   ring: all of the SM's shared memory when each CTA has an SM to itself.
+//   channels: 128, or fewer where that evens out one or two CTAs an SM.
 Int8Plan int8_tile_plan(const Int8Problem& p, int sms) {
   using S = Int8TileShape;
   Int8Plan pl;
-  const int64_t n_tiles = (p.N + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128);
+  pl.nr = p.gated ? 64 : 128;
+  int64_t n_tiles = (p.N + pl.nr - 1) / pl.nr;
   int64_t mn = 16;
   while (mn < S::MAX_MN && mn < p.M &&
          ((p.M + mn - 1) / mn > 1 && (mn < 32 || n_tiles * ((p.M + mn - 1) / mn) > 2 * sms)))
     mn *= 2;
   const int64_t m_tiles = (p.M + mn - 1) / mn;
   pl.mn = static_cast<int>(round_up((p.M + m_tiles - 1) / m_tiles, 16));
-  const int64_t tiles = n_tiles * m_tiles;
+  int64_t tiles = n_tiles * m_tiles;
   const int64_t k_blocks = (p.K + 127) / 128;
   const int64_t most = std::min<int64_t>(
       std::min<int64_t>(S::MAX_CLUSTER, 2 * sms / tiles),
       std::min<int64_t>(std::max<int64_t>(4, k_blocks / 6), k_blocks / 2));
   pl.cluster = most >= (m_tiles > 1 ? 3 : 2) ? static_cast<int>(most) : 1;
+  if (pl.cluster == 1 && tiles > sms && tiles <= 2 * sms) {
+    // One or two CTAs an SM: the channels per tile that leave the busiest SM least.
+    int64_t best = 2 * pl.nr;
+    for (int nr = pl.nr - 8; nr >= pl.nr / 2; nr -= 8) {
+      const int64_t t = (p.N + nr - 1) / nr * m_tiles;
+      if (t > 2 * sms) break;
+      if (2 * nr < best) {
+        best = 2 * nr;
+        pl.nr = nr;
+        tiles = t;
+      }
+    }
+  }
   const int room = tiles * pl.cluster <= sms ? S::FULL_SM : S::HALF_SM;
   pl.stages = std::min<int>(S::MAX_STAGES, (room - S::smem_bytes(pl.mn, 0)) / S::stage_bytes(pl.mn));
   return pl;
@@ -194,7 +210,7 @@ int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   auto kern = dx::int8_tile_kernel<T, G>;
   int rc = ensure_smem_attr(dev, reinterpret_cast<const void*>(kern), S::FULL_SM, true);
   if (rc) return rc;
-  constexpr int NT = G ? 64 : 128;
+  const int NT = pl.nr;
   CUtensorMap tW, tW2, tX;
   if ((rc = make_tmap_i8(&tW, pr.W, pr.K, pr.N, pr.ldw, NT, "W"))) return rc;
   if (G) {
@@ -217,6 +233,7 @@ int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.residual = pr.R;
   p.Y = pr.Y;
   p.act = pr.act;
+  p.nr = pl.nr;
   p.mn = pl.mn;
   p.stages = pl.stages;
   p.cluster = pl.cluster;
@@ -245,9 +262,9 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   if (rc) return rc;
   CUtensorMap tA, tB, tB2, tY, tR;
   if ((rc = make_tmap_i8(&tA, pr.X, pr.K, pr.M, pr.ldx, 128, "X"))) return rc;
-  if ((rc = make_tmap_i8(&tB, pr.W, pr.K, pr.N, pr.ldw, static_cast<uint32_t>(pl.bn / 2), "W"))) return rc;
+  if ((rc = make_tmap_i8(&tB, pr.W, pr.K, pr.N, pr.ldw, static_cast<uint32_t>(pl.bn / 4), "W"))) return rc;
   if (G) {
-    if ((rc = make_tmap_i8(&tB2, pr.W2, pr.K, pr.N, pr.ldw2, static_cast<uint32_t>(pl.bn / 2), "W2"))) return rc;
+    if ((rc = make_tmap_i8(&tB2, pr.W2, pr.K, pr.N, pr.ldw2, static_cast<uint32_t>(pl.bn / 4), "W2"))) return rc;
   } else {
     tB2 = tB;  // never read
   }
@@ -277,11 +294,14 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.has_residual = pr.R != nullptr ? 1 : 0;
   p.m_tiles = static_cast<int>((pr.M + 255) / 256);
   p.n_tiles = static_cast<int>((pr.N + NT - 1) / NT);
-  p.num_tiles = p.m_tiles * p.n_tiles;
+  const int tiles = p.m_tiles * p.n_tiles;
+  p.full_tiles = pl.halves ? tiles / pl.workers * pl.workers : tiles;
+  p.num_work = p.full_tiles + 2 * (tiles - p.full_tiles);
   p.group_m = pick_group_m(p.m_tiles, 256, (pr.K + 1) / 2);
-  p.workers = std::min(pl.workers, p.num_tiles);
-  set_plan("int8_pair%s tile=256x%d stages=%d grid=%d tiles=%d group_m=%d smem=%d",
-           G ? "_gated" : "", NT, p.stages, 2 * p.workers, p.num_tiles, p.group_m, S::SMEM_BYTES);
+  p.workers = std::min(pl.workers, p.num_work);
+  set_plan("int8_pair%s tile=256x%d stages=%d grid=%d tiles=%d full=%d group_m=%d smem=%d",
+           G ? "_gated" : "", NT, p.stages, 2 * p.workers, tiles, p.full_tiles, p.group_m,
+           S::SMEM_BYTES);
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg =
       launch_config(2 * p.workers, S::THREADS, S::SMEM_BYTES, pr.stream, 2, attr);
@@ -307,20 +327,26 @@ int dispatch_int8(const Int8Problem& p, int dev, const Int8Plan& pl) {
 // the last tile's epilogue, about bn, is not overlapped.  M = N = K = 4096: 45 us
 // at 256 (4 waves), 47 at 192 (5), 56 at 128 (7); M = 512: 12.4 at 128, 15.4 at
 // 256, 18.1 at 64 (2 waves); M = 3000, N = 5000: 43.5 at 224, 46 at 256.
-int int8_pair_bn(const Int8Problem& p, int workers) {
+// Where the tiles of the last wave fill at most half the pairs, they are done as
+// two halves of bn / 2 columns each: 3.7 waves' time instead of 4 for M = N = 4096.
+void int8_pair_tiles(const Int8Problem& p, int workers, Int8Plan* pl) {
   const int step = p.gated ? 64 : 32, wide = p.gated ? 2 : 1;
   const int64_t m_tiles = (p.M + 255) / 256;
-  int best = 256;
-  int64_t best_cost = -1;
+  auto wave = [](int bn) { return std::max(bn + 134, 268); };
+  int64_t best = -1;
   for (int bn = 256; bn >= 64; bn -= step) {
     const int64_t tiles = m_tiles * ((wide * p.N + bn - 1) / bn);
-    const int64_t cost = (tiles + workers - 1) / workers * std::max(bn + 134, 268) + bn;
-    if (best_cost < 0 || cost < best_cost) {
-      best_cost = cost;
-      best = bn;
+    const int64_t waves = tiles / workers, rest = tiles % workers;
+    int64_t cost = waves * wave(bn) + bn;
+    const bool halves = bn % (2 * step) == 0 && rest > 0 && 2 * rest <= workers &&
+                        waves > 0 && wave(bn / 2) < wave(bn);
+    if (rest > 0) cost += halves ? wave(bn / 2) - bn / 2 : wave(bn);
+    if (best < 0 || cost < best) {
+      best = cost;
+      pl->bn = bn;
+      pl->halves = halves;
     }
   }
-  return best;
 }
 
 // Pairs from 65 tokens on (us): M = 128, K = N = 4096: 11.5 against 12.3 for the
@@ -334,7 +360,7 @@ Int8Plan int8_plan(const Int8Problem& p, int dev, int sms) {
   if (slots < 1) return pl;
   pl.pair = true;
   pl.workers = slots;
-  pl.bn = int8_pair_bn(p, slots);
+  int8_pair_tiles(p, slots, &pl);
   return pl;
 }
 

@@ -150,6 +150,29 @@ def test_many_tiles(M, K, N):
         ref.check(int8_gated_linear(X, W, W2, b, kernel=kern), ref.gated(X, W, W2, b), kern)
 
 
+def _plan(key):
+    return int(nat.last_launch_plan().split(key + "=")[1].split()[0])
+
+
+@pytest.mark.parametrize("M,K,N", [(2560, 200, 2048), (4096, 128, 4040)])
+def test_last_wave_in_halves(M, K, N):
+    X, W, W2 = _x(M, K, torch.float16, 1), _w(N, K, 2), _w(N, K, 3)
+    b, R = _vec(N, torch.float16, 4), _x(M, N, torch.float16, 5)
+    ref.check(int8_linear(X, W, b, "relu", residual=R), ref.linear(X, W, b, "relu", R))
+    assert _plan("full") < _plan("tiles"), nat.last_launch_plan()
+    ref.check(int8_gated_linear(X, W, W2, b, None), ref.gated(X, W, W2, b, None))
+
+
+@pytest.mark.parametrize("N", [28672, 28601, 20000, 37888])
+def test_channels_per_tile_evened_out(N):
+    X, W = _x(9, 256, torch.bfloat16, 1), _w(N, 256, 2)
+    ref.check(int8_linear(X, W, None, "gelu_erf"), ref.linear(X, W, None, "gelu_erf"))
+    ref.check(int8_gated_linear(X, Int8Rows(W.q[:N // 2], W.scale[:N // 2]),
+                                int8_rows(W.q[N - N // 2:], W.scale[N - N // 2:])),
+              ref.gated(X, (W.q[:N // 2], W.scale[:N // 2]),
+                        (W.q[N - N // 2:], W.scale[N - N // 2:])))
+
+
 def test_extreme_integers_do_not_overflow():
     K = 131071
     q = torch.full((2, K), -128, dtype=torch.int8, device=DEV)
