@@ -157,18 +157,20 @@ struct Int8Plan {
   int nr = 128, mn = 16, cluster = 1, stages = 3;  // tile
 };
 
-// Tile kernel: tokens per tile, CTAs per cluster and ring depth (B200; us, W in
-// L2).  Two CTAs fit an SM, so a wave is 2 * SMs tiles.
+// Tile kernel: tokens and channels per tile, CTAs per cluster and ring depth (B200;
+// us, W in L2 unless it says otherwise).  Two CTAs fit an SM, so a wave is 2 * SMs tiles.
 //   tokens: the smallest of 16 / 32 / 64 / 128 whose tiles make one wave, then
 //   evened out.  M = 64, N = 4096: 10.0 with 32 a tile against 11.6 with 64;
 //   M = 512: 17.2 with 64, 19.3 with 128; M = 1024: 24.9 with 128 against 33.5
 //   with 64, which make two waves.
-//   cluster: as many CTAs as fill a wave, with some six K blocks each where there
-//   are that many.  M = 1, K = N = 4096: 6.3-6.6 for C = 5 to 8, 8.2 for 3, 11.6
-//   for 1; K = 14336: 11.3 for 7, 14.5 for 3; K = N = 1024: 4.0 for 4, 5.3 for 1.
-//   Beyond a wave it only costs: M = 16, N = 28672: 41 for 1, 45 for 2.
+//   cluster: as many CTAs as fill a wave, up to 6, with some six K blocks each where
+//   there are that many; none where the tiles alone keep two thirds of the SMs busy.
+//   M = 1, weights from HBM: K = N = 4096 6.6-6.9 us for C = 4 to 8, 7.0-7.5 for 3
+//   (11.6 for 1, in L2); K = 14336 13.5 for 5 and 6, 13.9 for 8, 14.4 for 3;
+//   K = N = 8192 14.7 for 3, 15.0 for 2, 18.3 for 1; N = 14336 12.9 for 1, 14.0 for 2.
 //   ring: all of the SM's shared memory when each CTA has an SM to itself.
-//   channels: 128, or fewer where that evens out one or two CTAs an SM.
+//   channels: 128, or fewer where that evens out one or two CTAs an SM
+//   (16 x 8192 x 28672: 40.2 us with 104 a tile, 41.5 with 128).
 Int8Plan int8_tile_plan(const Int8Problem& p, int sms) {
   using S = Int8TileShape;
   Int8Plan pl;
@@ -183,9 +185,9 @@ Int8Plan int8_tile_plan(const Int8Problem& p, int sms) {
   int64_t tiles = n_tiles * m_tiles;
   const int64_t k_blocks = (p.K + 127) / 128;
   const int64_t most = std::min<int64_t>(
-      std::min<int64_t>(S::MAX_CLUSTER, 2 * sms / tiles),
+      std::min<int64_t>(6, 2 * sms / tiles),
       std::min<int64_t>(std::max<int64_t>(4, k_blocks / 6), k_blocks / 2));
-  pl.cluster = most >= (m_tiles > 1 ? 3 : 2) ? static_cast<int>(most) : 1;
+  if (3 * tiles < 2 * sms && most >= (m_tiles > 1 ? 3 : 2)) pl.cluster = static_cast<int>(most);
   if (pl.cluster == 1 && tiles > sms && tiles <= 2 * sms) {
     // One or two CTAs an SM: the channels per tile that leave the busiest SM least.
     int64_t best = 2 * pl.nr;
