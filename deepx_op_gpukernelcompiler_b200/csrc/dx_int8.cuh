@@ -11,13 +11,12 @@
 //
 //   int8_pair_kernel  CTA pairs, 256 x bn tiles, persistent: the integer form
 //     of umma2_fused_linear_kernel (same roles, barriers and raster).  Serves
-//     problems with enough tiles to fill the GPU.
+//     more than 64 tokens.
 //   int8_tile_kernel  one 128 (channels) x mn (tokens) tile per CTA with the
 //     operands swapped — D^T[n, m] — so that a few tokens cost a narrow MMA
 //     while W streams past once; K split over a cluster of C CTAs that add
 //     their integer partial sums through distributed shared memory.  Integer
-//     sums do not depend on their order.  Serves decode, tall-skinny and
-//     ragged problems (its stores have no alignment rule).
+//     sums do not depend on their order.  Serves up to 64 tokens.
 //
 // Every mbarrier wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once
@@ -52,6 +51,7 @@ struct Int8Params {
   int full_tiles;  // tiles [full_tiles, m_tiles * n_tiles) are done as two halves each
   int num_work;    // full_tiles + 2 * the others
   int has_residual;
+  int tma_out;     // Y (and R) can be stored (and read) by TMA
 };
 
 __device__ __forceinline__ float ld_elem(const void* p, long long i, const __half*) {
@@ -383,6 +383,7 @@ struct Int8PairShape {
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int SMEM_BYTES = 1024 + OFF_MISC + 16;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static_assert(32 * 33 * 4 <= EPI_BUFS * kEpiBufBytes, "a chunk as fp32 rows");
 };
 
 // A pair's piece of work: a tile, or half the columns of one.
@@ -440,6 +441,39 @@ __device__ __forceinline__ void int8_scale(float (&v)[32], const uint32_t (&r)[3
   }
 }
 
+// 32 finished columns v of a warp's 32 rows (lane: row) into any Y: through shared
+// memory (33 floats a row: no bank conflicts), so that a store covers 32 columns
+// of one row.  For outputs that TMA cannot store: fp32, or rows that do not start on
+// 16 bytes.
+template <typename T>
+__device__ __forceinline__ void int8_store_rows(const Int8Params& p, const float (&v)[32], float* s,
+                                                int row0, int col, int lane) {
+  using Tr = ElemTraits<T>;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[lane * 33 + j] = v[j];
+  __syncwarp();
+  col += lane;
+  const int rows = col < p.N ? min(32, p.M - row0) : 0;
+  T* y = static_cast<T*>(p.Y) + row0 * p.ldy + col;
+  const T* res = static_cast<const T*>(p.residual);
+  if (res != nullptr) res += row0 * p.ldr + col;
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      x[r] = s[(r0 + r) * 33 + lane];
+      if (res != nullptr && r0 + r < rows) x[r] += Tr::to_float(res[r * p.ldr]);
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r0 + r < rows) y[r * p.ldy] = Tr::from_float(x[r]);
+    y += 8 * p.ldy;
+    if (res != nullptr) res += 8 * p.ldr;
+  }
+  __syncwarp();
+}
+
 template <typename T, bool kGated>
 __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
@@ -485,7 +519,7 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
     if (kGated) tma_prefetch_desc(&tmB2);
-    tma_prefetch_desc(&tmY);
+    if (p.tma_out) tma_prefetch_desc(&tmY);
     if (p.has_residual) tma_prefetch_desc(&tmR);
   }
   if (warp == 1) {
@@ -627,9 +661,10 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
           row_base < p.M && n0 < p.N ? min(chunks, (p.N - n0 + 31) / 32) : 0;
       // A chunk's staging buffer is free, and its residual on the way, one chunk
       // ahead (8192 x 14336 x 4096 with a residual: 363 us without).
-      if (live > 0) epi_chunk_begin<S::EPI_BUFS>(c, n0, row_base, lane, it);
+      const bool ahead = p.tma_out && live > 0;
+      if (ahead) epi_chunk_begin<S::EPI_BUFS>(c, n0, row_base, lane, it);
       if (!mbar_wait(bar(S::BAR_TFULL + b), use_ph, abort_flag)) {
-        if (live > 0) epi_chunk_drain<S::EPI_BUFS>(c, it);
+        if (ahead) epi_chunk_drain<S::EPI_BUFS>(c, it);
         break;
       }
       tc_fence_after();
@@ -649,7 +684,7 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
       bool ok = true;
 #pragma unroll 1
       for (int ch = 0; ch < live; ++ch) {
-        if (ch + 1 < live)
+        if (ahead && ch + 1 < live)
           epi_chunk_begin<S::EPI_BUFS>(c, n0 + 32 * (ch + 1), row_base, lane, it + 1);
         tmem_wait_ld();
         float v[32], w[32];
@@ -668,13 +703,20 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= w[j];
         }
-        if (!epi_chunk_store<S::EPI_BUFS>(c, v, n0 + 32 * ch, row_base, lane, it, abort_flag)) {
-          if (ch + 1 < live) {
-            tmem_wait_ld();
-            epi_chunk_drain<S::EPI_BUFS>(c, it + 1);
+        if (!ahead) {
+          int8_store_rows<T>(p, v, reinterpret_cast<float*>(c.ebuf_ptr0), row_base, n0 + 32 * ch,
+                             lane);
+          continue;
+        }
+        if constexpr (sizeof(T) == 2) {
+          if (!epi_chunk_store<S::EPI_BUFS>(c, v, n0 + 32 * ch, row_base, lane, it, abort_flag)) {
+            if (ch + 1 < live) {
+              tmem_wait_ld();
+              epi_chunk_drain<S::EPI_BUFS>(c, it + 1);
+            }
+            ok = false;
+            break;
           }
-          ok = false;
-          break;
         }
       }
       if (!ok) break;

@@ -144,8 +144,8 @@ int int8_validate(const Int8Problem& p) {
   return DX_OK;
 }
 
-// The pair kernel stores (and reads R) by TMA, in 16-bit types.
-bool int8_pair_eligible(const Int8Problem& p) {
+// Whether the pair kernel can store Y (and read R) by TMA.
+bool int8_tma_out(const Int8Problem& p) {
   return p.dtype != DX_DTYPE_F32 && tma_ok(p.Y, p.ldy) && (p.R == nullptr || tma_ok(p.R, p.ldr));
 }
 
@@ -271,9 +271,14 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
     tB2 = tB;  // never read
   }
   const CUtensorMapDataType dt = tma_dtype(pr.dtype);
-  if ((rc = make_tmap_2d(&tY, pr.Y, dt, pr.N, pr.M, pr.ldy, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, "Y")))
+  const bool tma_out = int8_tma_out(pr);
+  if (!tma_out) {
+    tY = tA;  // never read
+  } else if ((rc = make_tmap_2d(&tY, pr.Y, dt, pr.N, pr.M, pr.ldy, 32, 32,
+                                CU_TENSOR_MAP_SWIZZLE_64B, "Y"))) {
     return rc;
-  if (pr.R != nullptr) {
+  }
+  if (tma_out && pr.R != nullptr) {
     if ((rc = make_tmap_2d(&tR, pr.R, dt, pr.N, pr.M, pr.ldr, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B,
                            "R")))
       return rc;
@@ -293,7 +298,12 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.bias = pr.bias;
   p.bias2 = pr.bias2;
   p.act = pr.act;
-  p.has_residual = pr.R != nullptr ? 1 : 0;
+  p.tma_out = tma_out ? 1 : 0;
+  p.has_residual = tma_out && pr.R != nullptr ? 1 : 0;
+  p.residual = pr.R;
+  p.ldr = pr.ldr;
+  p.Y = pr.Y;
+  p.ldy = pr.ldy;
   p.m_tiles = static_cast<int>((pr.M + 255) / 256);
   p.n_tiles = static_cast<int>((pr.N + NT - 1) / NT);
   const int tiles = p.m_tiles * p.n_tiles;
@@ -301,8 +311,8 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.num_work = p.full_tiles + 2 * (tiles - p.full_tiles);
   p.group_m = pick_group_m(p.m_tiles, 256, (pr.K + 1) / 2);
   p.workers = std::min(pl.workers, p.num_work);
-  set_plan("int8_pair%s tile=256x%d stages=%d grid=%d tiles=%d full=%d group_m=%d smem=%d",
-           G ? "_gated" : "", NT, p.stages, 2 * p.workers, tiles, p.full_tiles, p.group_m,
+  set_plan("int8_pair%s tile=256x%d tma_out=%d stages=%d grid=%d tiles=%d full=%d group_m=%d smem=%d",
+           G ? "_gated" : "", NT, p.tma_out, p.stages, 2 * p.workers, tiles, p.full_tiles, p.group_m,
            S::SMEM_BYTES);
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg =
@@ -315,9 +325,11 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
 
 template <bool G>
 int dispatch_int8(const Int8Problem& p, int dev, const Int8Plan& pl) {
-  if (pl.pair)
+  if (pl.pair) {
+    if (p.dtype == DX_DTYPE_F32) return launch_int8_pair<float, G>(p, dev, pl);
     return p.dtype == DX_DTYPE_F16 ? launch_int8_pair<__half, G>(p, dev, pl)
                                    : launch_int8_pair<__nv_bfloat16, G>(p, dev, pl);
+  }
   if (p.dtype == DX_DTYPE_F32) return launch_int8_tile<float, G>(p, dev, pl);
   return p.dtype == DX_DTYPE_F16 ? launch_int8_tile<__half, G>(p, dev, pl)
                                  : launch_int8_tile<__nv_bfloat16, G>(p, dev, pl);
@@ -356,8 +368,7 @@ void int8_pair_tiles(const Int8Problem& p, int workers, Int8Plan* pl) {
 // N = 14336 17.9 against 14.2.
 Int8Plan int8_plan(const Int8Problem& p, int dev, int sms) {
   Int8Plan pl = int8_tile_plan(p, sms);
-  if (p.kernel == DX_KERNEL_DECODE || !int8_pair_eligible(p)) return pl;
-  if (p.kernel == DX_KERNEL_AUTO && p.M <= 64) return pl;
+  if (p.kernel == DX_KERNEL_DECODE || (p.kernel == DX_KERNEL_AUTO && p.M <= 64)) return pl;
   const int slots = std::min(pair_slots<256, __nv_bfloat16>(dev, sms), sms / 2);
   if (slots < 1) return pl;
   pl.pair = true;
@@ -371,10 +382,6 @@ int run_int8(Int8Problem& p) {
   int rc = int8_validate(p);
   if (rc) return rc;
   if (p.M == 0 || p.N == 0) return DX_OK;
-  if (p.kernel == DX_KERNEL_UMMA && !int8_pair_eligible(p))
-    return fail(DX_ERR_UNSUPPORTED,
-                "the CTA-pair kernel needs a 16-bit output and 16-byte-aligned Y and R with row "
-                "pitches that are multiples of 16 bytes");
   if (p.x_dtype != DX_DTYPE_I8) {
     const size_t need = int8_workspace(p.M, p.K);
     if (p.ws == nullptr || p.ws_bytes < need || !aligned16(p.ws))

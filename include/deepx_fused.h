@@ -305,8 +305,9 @@ int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K,
  * needs no initial value).  bias, R and Y have type `dtype`; W is
  * 16-byte-aligned with ldw a multiple of 16.  The sums are exact (32-bit
  * integers, 1 <= K <= 131071) and become fp32 once.  `kernel` is
- * DX_KERNEL_AUTO, DX_KERNEL_UMMA (CTA pairs; 16-bit outputs whose rows are
- * 16-byte aligned) or DX_KERNEL_DECODE (one tile per CTA, any output).
+ * DX_KERNEL_AUTO, DX_KERNEL_UMMA (CTA pairs) or DX_KERNEL_DECODE (one tile per
+ * CTA, K split over a cluster).  Outputs of the CTA pairs whose rows are 16-byte
+ * aligned and 16-bit are stored by TMA; others go a row at a time.
  */
 int dx_int8_linear(const void* X, int x_dtype, const float* x_scale, const void* W,
                    const float* w_scale, const void* bias, const void* R, void* Y, int64_t M,

@@ -96,6 +96,10 @@ def test_quantize_weight_is_per_channel():
     assert (r.dequantize().cpu().t() - W.float().cpu()).abs().max() <= s.max() * 0.5001
 
 
+def _plan(key):
+    return int(nat.last_launch_plan().split(key + "=")[1].split()[0])
+
+
 # ---------------------------------------------------------------- products
 SHAPES = [  # M, K, N
     (1, 1, 1), (1, 128, 128), (1, 4096, 512), (2, 130, 77), (7, 1000, 300), (16, 4096, 1024),
@@ -117,10 +121,10 @@ def test_linear(M, K, N, dtype):
     ref.check(plain, ref.linear(X, W), "tile")
     pair = quantize_rows(X)
     ref.check(int8_linear(pair, W, b, act, dtype=dt), ref.linear(X, W, b, act), "8-bit X")
-    if dtype != "f32" and N % 8 == 0:
-        Y = int8_linear(X, W, b, act, residual=R, kernel="umma")
-        assert nat.last_launch_plan().startswith("int8_pair"), nat.last_launch_plan()
-        ref.check(Y, ref.linear(X, W, b, act, R), "pair")
+    Y = int8_linear(X, W, b, act, residual=R, kernel="umma")
+    assert nat.last_launch_plan().startswith("int8_pair"), nat.last_launch_plan()
+    assert _plan("tma_out") == (dtype != "f32" and N % 8 == 0)
+    ref.check(Y, ref.linear(X, W, b, act, R), "pair")
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -134,24 +138,20 @@ def test_gated(M, K, N, dtype):
     ref.check(int8_gated_linear(X, Wg, Wu, None, bu, act, kernel="decode"),
               ref.gated(X, Wg, Wu, None, bu, act), "tile")
     assert nat.last_launch_plan().startswith("int8_tile_gated"), nat.last_launch_plan()
-    if dtype != "f32" and N % 8 == 0:
-        Y = int8_gated_linear(quantize_rows(X), Wg, Wu, bg, None, act, kernel="umma", dtype=dt)
-        assert nat.last_launch_plan().startswith("int8_pair_gated"), nat.last_launch_plan()
-        ref.check(Y, ref.gated(X, Wg, Wu, bg, None, act), "pair")
+    Y = int8_gated_linear(quantize_rows(X), Wg, Wu, bg, None, act, kernel="umma", dtype=dt)
+    assert nat.last_launch_plan().startswith("int8_pair_gated"), nat.last_launch_plan()
+    ref.check(Y, ref.gated(X, Wg, Wu, bg, None, act), "pair")
 
 
-@pytest.mark.parametrize("M,K,N", [(600, 384, 2100), (1024, 520, 4096), (2048, 130, 2568)])
+@pytest.mark.parametrize("M,K,N", [(600, 384, 2100), (1024, 520, 4096), (2048, 130, 2568),
+                                   (1500, 96, 5003)])
 def test_many_tiles(M, K, N):
     """More tiles than a wave of CTA pairs, and raster groups of several m-tiles."""
     X, W, W2 = _x(M, K, torch.bfloat16, 1), _w(N, K, 2), _w(N, K, 3)
     b = _vec(N, torch.bfloat16, 4)
-    for kern in ("auto", "umma", "decode") if N % 8 == 0 else ("auto", "decode"):
+    for kern in ("auto", "umma", "decode"):
         ref.check(int8_linear(X, W, b, "silu", kernel=kern), ref.linear(X, W, b, "silu"), kern)
         ref.check(int8_gated_linear(X, W, W2, b, kernel=kern), ref.gated(X, W, W2, b), kern)
-
-
-def _plan(key):
-    return int(nat.last_launch_plan().split(key + "=")[1].split()[0])
 
 
 @pytest.mark.parametrize("M,K,N", [(2560, 200, 2048), (4096, 128, 4040)])

@@ -45,8 +45,6 @@ def _linear(lib, **kw):
     (dict(R=FAKE, ldr=2), nat.DX_ERR_INVALID_ARGUMENT, "ldr"),
     (dict(ldw=40), nat.DX_ERR_UNSUPPORTED, "16-byte"),
     (dict(X=FAKE + 8), nat.DX_ERR_UNSUPPORTED, "16-byte"),
-    (dict(kernel=nat.DX_KERNEL_UMMA, dtype=nat.DX_DTYPE_F32), nat.DX_ERR_UNSUPPORTED, "16-bit"),
-    (dict(kernel=nat.DX_KERNEL_UMMA, ldy=33), nat.DX_ERR_UNSUPPORTED, "16-byte"),
     (dict(x_dtype=nat.DX_DTYPE_BF16), nat.DX_ERR_WORKSPACE, "workspace"),
 ])
 def test_linear_host_validation(lib, kw, code, needle):
