@@ -418,12 +418,48 @@ __device__ __forceinline__ void int8_tile_coords(const Int8Params& p, int t, int
   nb = r / gm;
 }
 
-// `cols` column values from n (zeros past N) to a warp's shared array.
-template <typename E>
-__device__ __forceinline__ void int8_stage_vec(float* dst, const E* src, int n, int cols, int N,
-                                               int lane) {
-  for (int j = lane; j < cols; j += 32)
-    dst[j] = (src != nullptr && n + j < N) ? ElemTraits<E>::to_float(src[n + j]) : 0.0f;
+// Scales and biases of a warp's columns, spread over its lanes: a register holds
+// column lane + 32 k.  Asked for one tile ahead (short K loops do not hide the
+// trip to memory), then put into the warp's shared arrays.
+template <bool kGated>
+struct Int8Columns {
+  static constexpr int kPer = kGated ? 2 : 4;  // at most 64 / 128 columns
+  float t[kPer], b[kPer], t2[kGated ? kPer : 1], b2[kGated ? kPer : 1];
+  float sx;  // of the lane's row
+};
+
+template <typename T, bool kGated>
+__device__ __forceinline__ void int8_fetch_columns(const Int8Params& p, int n, int cols, int row,
+                                                   int lane, Int8Columns<kGated>& c) {
+  const T* const bias = static_cast<const T*>(p.bias);
+  const T* const bias2 = static_cast<const T*>(p.bias2);
+  c.sx = row < p.M ? p.sx[row] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < Int8Columns<kGated>::kPer; ++k) {
+    const int j = n + lane + 32 * k;
+    const bool in = 32 * k < cols && j < p.N;
+    c.t[k] = in ? p.sw[j] : 0.0f;
+    c.b[k] = in && bias != nullptr ? ElemTraits<T>::to_float(bias[j]) : 0.0f;
+    if (kGated) {
+      c.t2[k] = in ? p.sw2[j] : 0.0f;
+      c.b2[k] = in && bias2 != nullptr ? ElemTraits<T>::to_float(bias2[j]) : 0.0f;
+    }
+  }
+}
+
+template <bool kGated>
+__device__ __forceinline__ void int8_put_columns(const Int8Columns<kGated>& c, float* vec, int lane) {
+  __syncwarp();  // the previous tile's values are no longer read
+#pragma unroll
+  for (int k = 0; k < Int8Columns<kGated>::kPer; ++k) {
+    vec[lane + 32 * k] = c.t[k];
+    vec[128 + lane + 32 * k] = c.b[k];
+    if (kGated) {
+      vec[256 + lane + 32 * k] = c.t2[k];
+      vec[384 + lane + 32 * k] = c.b2[k];
+    }
+  }
+  __syncwarp();
 }
 
 // v = acc * (sx * t) + b over the 32 columns at t, b (shared memory, read as
@@ -456,20 +492,28 @@ __device__ __forceinline__ void int8_store_rows(const Int8Params& p, const float
   const int rows = col < p.N ? min(32, p.M - row0) : 0;
   T* y = static_cast<T*>(p.Y) + row0 * p.ldy + col;
   const T* res = static_cast<const T*>(p.residual);
-  if (res != nullptr) res += row0 * p.ldr + col;
-#pragma unroll 1
-  for (int r0 = 0; r0 < rows; r0 += 8) {
-    float x[8];
+  if (rows == 32 && res == nullptr) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      x[r] = s[(r0 + r) * 33 + lane];
-      if (res != nullptr && r0 + r < rows) x[r] += Tr::to_float(res[r * p.ldr]);
+    for (int r = 0; r < 32; ++r) {
+      *y = Tr::from_float(s[r * 33 + lane]);
+      y += p.ldy;
     }
+  } else {
+    if (res != nullptr) res += row0 * p.ldr + col;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+      float x[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r0 + r < rows) y[r * p.ldy] = Tr::from_float(x[r]);
-    y += 8 * p.ldy;
-    if (res != nullptr) res += 8 * p.ldr;
+      for (int r = 0; r < 8; ++r) {
+        x[r] = s[(r0 + r) * 33 + lane];
+        if (res != nullptr && r0 + r < rows) x[r] += Tr::to_float(res[r * p.ldr]);
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r0 + r < rows) y[r * p.ldy] = Tr::from_float(x[r]);
+      y += 8 * p.ldy;
+      if (res != nullptr) res += 8 * p.ldr;
+    }
   }
   __syncwarp();
 }
@@ -636,27 +680,34 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
     float* const vec = reinterpret_cast<float*>(base_ptr + S::OFF_VEC + e * S::VEC_BYTES);
     uint32_t it = 0;
     int local = 0;
+    // Where this warp works on the i'th piece: its first column and 32-column chunks
+    // (half of the piece's), and the first of its 32 rows.
+    auto place = [&](int i, Int8Work& wk, int& n0, int& c0, int& chunks, int& row_base) {
+      wk = int8_work(p, i);
+      const int out_cols = kGated ? wk.bn / 2 : wk.bn;
+      const int half = (out_cols / 32 + 1) / 2;
+      c0 = (e / 4) * half * 32;
+      chunks = e / 4 == 0 ? half : out_cols / 32 - half;
+      n0 = wk.nb * (kGated ? p.bn / 2 : p.bn) + wk.half * out_cols + c0;
+      row_base = wk.mb * 2 * S::BM + static_cast<int>(rank) * S::BM + q * 32;
+    };
+    Int8Work wk;
+    int n0, c0, chunks, row_base;
+    Int8Columns<kGated> cols;
+    if (pair < p.num_work) {
+      place(pair, wk, n0, c0, chunks, row_base);
+      int8_fetch_columns<T, kGated>(p, n0, 32 * chunks, row_base + lane, lane, cols);
+    }
     for (int i = pair; i < p.num_work; i += p.workers, ++local) {
       const int b = local & 1;
       const uint32_t use_ph = (static_cast<uint32_t>(local) >> 1) & 1u;
-      const Int8Work wk = int8_work(p, i);
-      // Output columns of the work, and this warp's half of their 32-column chunks.
-      const int out_cols = kGated ? wk.bn / 2 : wk.bn;
-      const int half = (out_cols / 32 + 1) / 2;
-      const int c0 = (e / 4) * half * 32;
-      const int chunks = e / 4 == 0 ? half : out_cols / 32 - half;
-      const int n0 = wk.nb * (kGated ? p.bn / 2 : p.bn) + wk.half * out_cols + c0;
-      const int row_base = wk.mb * 2 * S::BM + static_cast<int>(rank) * S::BM + q * 32;
-      const int row = row_base + lane;
-      const float sx = row < p.M ? p.sx[row] : 0.0f;
-      __syncwarp();  // the previous tile's values are no longer read
-      int8_stage_vec(vec, p.sw, n0, 32 * chunks, p.N, lane);
-      int8_stage_vec(vec + 128, static_cast<const T*>(p.bias), n0, 32 * chunks, p.N, lane);
-      if (kGated) {
-        int8_stage_vec(vec + 256, p.sw2, n0, 32 * chunks, p.N, lane);
-        int8_stage_vec(vec + 384, static_cast<const T*>(p.bias2), n0, 32 * chunks, p.N, lane);
+      const float sx = cols.sx;
+      int8_put_columns<kGated>(cols, vec, lane);
+      if (i + p.workers < p.num_work) {
+        place(i + p.workers, wk, n0, c0, chunks, row_base);
+        int8_fetch_columns<T, kGated>(p, n0, 32 * chunks, row_base + lane, lane, cols);
       }
-      __syncwarp();
+      place(i, wk, n0, c0, chunks, row_base);
       const int live =
           row_base < p.M && n0 < p.N ? min(chunks, (p.N - n0 + 31) / 32) : 0;
       // A chunk's staging buffer is free, and its residual on the way, one chunk
