@@ -33,6 +33,8 @@
 // Every wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once
 
+#include <type_traits>
+
 #include "dx_epilogue.cuh"
 #include "dx_ptx.cuh"
 
@@ -41,6 +43,7 @@ namespace dx {
 constexpr int kMoeMaxT = 64;
 constexpr int kMoeMaxE = 256;
 constexpr int kMoeMaxTop = 32;
+constexpr int kMoeWholeBlocks = 10;
 
 // ---------------------------------------------------------------- router
 constexpr int kRouterThreads = 1024;
@@ -334,8 +337,12 @@ __device__ __forceinline__ MoePhase moe_phase(const MoeParams& p, int chosen, bo
   f.per_tile = second ? chosen * p.kb_h : p.kb_d;
   f.tiles = second ? p.nt_d : chosen * p.nt_h;
   f.whole = f.tiles / grid * grid;
+  // Fewer tiles than CTAs, and short ones: joining partial sums (some 5 us) costs more
+  // than the K blocks it saves the CTAs that have a tile (some 0.5 us each).
+  if (!second && f.whole == 0 && f.per_tile - f.tiles * f.per_tile / grid <= kMoeWholeBlocks)
+    f.whole = f.tiles;
   f.units = (f.tiles - f.whole) * f.per_tile;
-  f.ctas = min(grid, f.units);
+  f.ctas = min(grid, f.units);  // (0: no split tiles)
   f.u0 = g < f.ctas ? f.begin(g) : 0;
   f.u1 = g < f.ctas ? f.begin(g + 1) : 0;
   return f;
@@ -671,32 +678,39 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         atomicAdd(ctr, 1);
         *s_ok = share < 0 || moe_wait(ctr, peers, abort_flag) ? 1 : 0;
       }
-      named_bar_sync(1, 128);
-      __threadfence();
+      named_bar_sync(1, 128);  // (behind it the partials are read from L2, past L1)
       return *s_ok != 0;
     };
-    // Columns 4 lane .. 4 lane + 3 of row `row` of the tile, added in CTA order.
-    auto row_sum = [&](int row) {
+    // Columns 4 lane .. 4 lane + 3 of kRows rows of the tile, `apart` rows apart, added
+    // in CTA order.
+    auto row_sums = [&](auto rows, int row, int apart, float4* t) {
+      constexpr int kRows = decltype(rows)::value, kBatch = 8 / kRows;
       const long long at = static_cast<long long>(row) * 128 + 4 * lane;
-      float4 t = __ldcg(reinterpret_cast<const float4*>(sum + at));
       const float* const next = part(first + 1, 0) + at;
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        t[j] = __ldcg(reinterpret_cast<const float4*>(sum + at + j * apart * 128));
 #pragma unroll 1
-      for (int i = 0; i < peers - 1; i += 8) {
-        float4 v[8];
+      for (int i = 0; i < peers - 1; i += kBatch) {
+        float4 v[kBatch][kRows];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          v[k] = i + k < peers - 1
-                     ? __ldcg(reinterpret_cast<const float4*>(next + 2 * slot_floats * (i + k)))
-                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < kBatch; ++k)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          t.x += v[k].x;
-          t.y += v[k].y;
-          t.z += v[k].z;
-          t.w += v[k].w;
-        }
+          for (int j = 0; j < kRows; ++j)
+            v[k][j] = i + k < peers - 1
+                          ? __ldcg(reinterpret_cast<const float4*>(
+                                next + 2 * slot_floats * (i + k) + j * apart * 128))
+                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            t[j].x += v[k][j].x;
+            t[j].y += v[k][j].y;
+            t[j].z += v[k][j].z;
+            t[j].w += v[k][j].w;
+          }
       }
-      return t;
     };
 
     {  // ---- phase 1: h
@@ -768,9 +782,10 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         for (unsigned long long left = mask; left != 0; left &= left - 1, ++i) {
           if (i % (4 * shares) != share * 4 + q) continue;
           const int m = __ffsll(static_cast<long long>(left)) - 1;
-          const float4 ga = row_sum(m), up = row_sum(p.T + m);
+          float4 t[2];  // gate, up
+          row_sums(std::integral_constant<int, 2>(), m, p.T, t);
           if (col >= p.H) continue;
-          float v[4] = {ga.x, ga.y, ga.z, ga.w}, w[4] = {up.x, up.y, up.z, up.w};
+          float v[4] = {t[0].x, t[0].y, t[0].z, t[0].w}, w[4] = {t[1].x, t[1].y, t[1].z, t[1].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             v[k] += moe_bias(bg, bi + k);
@@ -868,7 +883,8 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         // This CTA's share of the rows (halves of a token's 256 columns), a warp each.
 #pragma unroll 1
         for (int row = share * 4 + q; row < 2 * p.T; row += 4 * shares) {
-          const float4 t = row_sum(row);
+          float4 t;
+          row_sums(std::integral_constant<int, 1>(), row, 0, &t);
           const int h = row >= p.T ? 1 : 0, m = row - h * p.T;
           const int c = r.tile * 256 + 128 * h + 4 * lane;
           if (c >= p.D) continue;

@@ -12,30 +12,42 @@ Wo [E, H, D].  A shared expert's output, or the residual stream, goes in as
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from . import _native as nat
 from .int8 import _like, _on_device
-from .linear import DTYPE_CODES, _check_matrix, _ld, activation_code
+from .linear import DTYPE_CODES as _CODES
+from .linear import _check_matrix, _ld, activation_code
 
 MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 256, 32
 
 
-def _experts(name: str, W: torch.Tensor, shape: tuple, X: torch.Tensor) -> None:
-    if W.dim() != 3 or tuple(W.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(W.shape)}")
+# dx_moe_args packed by struct: a third of the time of filling a ctypes.Structure
+# (13 pointers, 15 int64, 3 int, padding, pointer, size_t).
+_PACK = struct.Struct("@13P15q3i4xPN")
+assert _PACK.size == ctypes.sizeof(nat.MoeArgs)
+
+
+def _experts(name: str, W: torch.Tensor, E: int, rows: int, cols: int, X: torch.Tensor,
+             index: int):
+    """Checks stacked expert weights -> (address, row pitch, expert pitch)."""
+    if W.shape != (E, rows, cols):
+        raise ValueError(f"{name} must have shape {(E, rows, cols)}, got {tuple(W.shape)}")
     se, sr, sc = W.stride()
-    if sc != 1 or sr < shape[2] or (shape[0] > 1 and se < sr * shape[1]):
+    if sc != 1 or sr < cols or (E > 1 and se < sr * rows):
         raise ValueError(f"{name} must be [E, rows, columns] with contiguous rows that do not "
                          f"overlap, got strides {W.stride()}")
-    _like(name, W, X, X.dtype)
+    if W.dtype is not X.dtype or W.get_device() != index:
+        _like(name, W, X, X.dtype)
+    return W.data_ptr(), sr, se
 
 
-def _bias(name: str, b: torch.Tensor | None, shape: tuple, X: torch.Tensor):
+def _bias(name: str, b: torch.Tensor | None, shape: tuple, X: torch.Tensor) -> int:
     if b is None:
-        return None
-    if tuple(b.shape) != shape or not b.is_contiguous():
+        return 0
+    if b.shape != shape or not b.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of shape {shape}, got "
                          f"{tuple(b.shape)}")
     _like(name, b, X, X.dtype)
@@ -58,9 +70,9 @@ def moe_ffn(X: torch.Tensor, Wr: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tenso
     act = activation_code(activation)
     if not isinstance(X, torch.Tensor):
         raise TypeError("X must be a torch tensor")
-    code = DTYPE_CODES.get(X.dtype)
-    if X.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"unsupported dtype {X.dtype}; moe_ffn takes float16 or bfloat16")
+    dtype = X.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"unsupported dtype {dtype}; moe_ffn takes float16 or bfloat16")
     _check_matrix("X", X, None, None)
     T, D = X.shape
     _check_matrix("Wr", Wr, D, None)
@@ -76,28 +88,34 @@ def moe_ffn(X: torch.Tensor, Wr: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tenso
         raise ValueError(f"top_k must be between 1 and {min(E, MAX_TOP_K)}, got {top_k}")
     if D % 8 or H % 8 or not D or not H:
         raise ValueError(f"D and H must be multiples of 8, got {D} and {H}")
-    _like("Wr", Wr, X, X.dtype)
-    _experts("Wg", Wg, (E, D, H), X)
-    _experts("Wu", Wu, (E, D, H), X)
-    _experts("Wo", Wo, (E, H, D), X)
+    _like("Wr", Wr, X, dtype)
+    index = X.get_device()
+    wg, ldg, ldg_e = _experts("Wg", Wg, E, D, H, X, index)
+    wu, ldu, ldu_e = _experts("Wu", Wu, E, D, H, X, index)
+    wo, ldo, ldo_e = _experts("Wo", Wo, E, H, D, X, index)
     br_ptr, bg_ptr = _bias("br", br, (E,), X), _bias("bg", bg, (E, H), X)
     bu_ptr, bo_ptr = _bias("bu", bu, (E, H), X), _bias("bo", bo, (E, D), X)
-    r_ptr, ldr = None, 0
+    r_ptr = ldr = 0
     if residual is not None:
         _check_matrix("residual", residual, T, D)
-        _like("residual", residual, X, X.dtype)
+        _like("residual", residual, X, dtype)
         r_ptr, ldr = residual.data_ptr(), _ld(residual)
-    if X.device.type != "cuda":
+    if not X.is_cuda:
         raise ValueError("moe_ffn runs on CUDA tensors only (the engine has no CPU path)")
     if out is None:
-        out = X.new_empty((T, D))
+        out, ldy = X.new_empty((T, D)), D
     else:
         _check_matrix("out", out, T, D)
-        _like("out", out, X, X.dtype)
-    if X.data_ptr() % 16 or (T > 1 and X.stride(0) % 8):
-        X = X.contiguous() if not X.is_contiguous() else X.clone()
-    routing = X.new_empty((2, T, top_k), dtype=torch.float32)
-    weights, ids = routing[0], routing[1].view(torch.int32)
+        _like("out", out, X, dtype)
+        ldy = _ld(out)
+    x_ptr, ldx = X.data_ptr(), _ld(X)
+    if x_ptr % 16 or (T > 1 and ldx % 8):
+        X = X.clone(memory_format=torch.contiguous_format)
+        x_ptr, ldx = X.data_ptr(), D
+    if T == 1:
+        ldx = D
+    weights = X.new_empty((T, top_k), dtype=torch.float32)
+    ids = X.new_empty((T, top_k), dtype=torch.int32)
     lib = nat.load()
 
     def call(stream):
@@ -105,15 +123,13 @@ def moe_ffn(X: torch.Tensor, Wr: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tenso
         # graph being captured.
         size = lib.dx_moe_workspace_size(T, H, E, top_k)
         space = X.new_empty(size, dtype=torch.uint8)
-        args = nat.MoeArgs(
-            X.data_ptr(), Wr.data_ptr(), br_ptr, Wg.data_ptr(), Wu.data_ptr(), Wo.data_ptr(),
-            bg_ptr, bu_ptr, bo_ptr, r_ptr, out.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, D,
-            H, E, top_k, _ld(X), _ld(Wr), Wg.stride(1), Wg.stride(0), Wu.stride(1), Wu.stride(0),
-            Wo.stride(1), Wo.stride(0), ldr, _ld(out), code, act, 1 if renormalize else 0,
-            space.data_ptr(), size)
-        return lib.dx_moe(ctypes.addressof(args), stream)
+        return lib.dx_moe(_PACK.pack(
+            x_ptr, Wr.data_ptr(), br_ptr, wg, wu, wo, bg_ptr, bu_ptr, bo_ptr, r_ptr,
+            out.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, D, H, E, top_k, ldx, _ld(Wr),
+            ldg, ldg_e, ldu, ldu_e, ldo, ldo_e, ldr, ldy, _CODES[dtype], act,
+            1 if renormalize else 0, space.data_ptr(), size), stream)
 
-    rc = _on_device(X.get_device(), call)
+    rc = _on_device(index, call)
     if rc:
         nat.check("dx_moe", rc)
     return (out, weights, ids) if return_routing else out
