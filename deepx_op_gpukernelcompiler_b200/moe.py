@@ -41,7 +41,7 @@ def _experts(name: str, W: torch.Tensor, E: int, rows: int, cols: int, X: torch.
                          f"overlap, got strides {W.stride()}")
     if W.dtype is not X.dtype or W.get_device() != index:
         _like(name, W, X, X.dtype)
-    return W.data_ptr(), sr, se
+    return W.data_ptr(), sr, se if E > 1 else sr * rows
 
 
 def _bias(name: str, b: torch.Tensor | None, shape: tuple, X: torch.Tensor) -> int:
@@ -66,7 +66,10 @@ def moe_ffn(X: torch.Tensor, Wr: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tenso
     goes to the top_k experts of the largest logits X Wr + br (ties: the lowest
     number); w is the softmax over them, or over all experts with
     ``renormalize=False``.  With ``return_routing`` the result is (Y, w [T, top_k]
-    float32, expert numbers [T, top_k] int32), largest first."""
+    float32, expert numbers [T, top_k] int32), largest first.  What an expert
+    computes reaches only the tokens that chose it.  The hidden values pass between
+    the two products as a pair of 16-bit values each (hi + lo), so they are as exact
+    as fp32 ones, but in float16 they must stay below 65504."""
     act = activation_code(activation)
     if not isinstance(X, torch.Tensor):
         raise TypeError("X must be a torch tensor")

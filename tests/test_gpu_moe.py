@@ -134,6 +134,15 @@ def test_strided_operands_untouched_rows_and_in_place():
     ref.check(got, ref.moe(**t, top_k=2, residual=t["X"]), "in place")
 
 
+def test_one_expert_given_by_a_view():
+    """E = 1: the expert pitch of a view plays no part."""
+    t = make(3, 64, 40, 1, torch.bfloat16)
+    for name in ("Wg", "Wu", "Wo"):
+        t[name] = t[name][0].as_strided((1, *t[name].shape[1:]), (0, t[name].shape[2], 1))
+    got = moe_ffn(**t, top_k=1, return_routing=True)
+    ref.check(got, ref.moe(**t, top_k=1))
+
+
 def test_empty_batch():
     t = make(1, 64, 64, 4, torch.bfloat16)
     t["X"] = t["X"][:0]
