@@ -40,29 +40,29 @@ int make_tmap_i8(CUtensorMap* m, const void* ptr, int64_t k, int64_t rows, int64
 }
 
 // ---------------------------------------------------------- quantisation
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool kVec>
 int launch_quantize(const QuantParams& p, int sms, cudaStream_t s) {
   // 1024 threads an SM, each CTA taking every grid'th row.
   const int grid = std::min(p.M, sms * (1024 / THREADS));
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = launch_config(grid, THREADS, 0, s, 1, attr);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, dx::quantize_rows_kernel<T, THREADS>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, dx::quantize_rows_kernel<T, THREADS, kVec>, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch quantize_rows_kernel");
   return DX_OK;
 }
 
-template <typename T>
+template <typename T, bool kVec>
 int quantize_typed(const QuantParams& p, int sms, cudaStream_t s) {
   // Few rows: the latency of a row counts, one vector a thread; many: all that
   // its registers hold, so that a row takes few threads and many are in flight.
   constexpr int kRegs = dx::kQuantRegsOf<T>;
   const int vectors = (p.K + dx::kQuantVec - 1) / dx::kQuantVec;
   const int threads = p.M <= 4 * sms ? vectors : (vectors + kRegs - 1) / kRegs;
-  if (threads <= 128) return launch_quantize<T, 128>(p, sms, s);
-  if (threads <= 256) return launch_quantize<T, 256>(p, sms, s);
-  if (threads <= 512) return launch_quantize<T, 512>(p, sms, s);
-  return launch_quantize<T, 1024>(p, sms, s);
+  if (threads <= 128) return launch_quantize<T, 128, kVec>(p, sms, s);
+  if (threads <= 256) return launch_quantize<T, 256, kVec>(p, sms, s);
+  if (threads <= 512) return launch_quantize<T, 512, kVec>(p, sms, s);
+  return launch_quantize<T, 1024, kVec>(p, sms, s);
 }
 
 int run_quantize(const void* X, void* Q, float* scale, int64_t M, int64_t K, int64_t ldx,
@@ -75,10 +75,14 @@ int run_quantize(const void* X, void* Q, float* scale, int64_t M, int64_t K, int
   p.K = static_cast<int>(K);
   p.ldx = ldx;
   p.ldq = ldq;
-  p.vec = aligned16(X) && (ldx * elem_size(dtype)) % 16 == 0 && aligned16(Q) && ldq % 8 == 0;
-  if (dtype == DX_DTYPE_F32) return quantize_typed<float>(p, sms, s);
-  if (dtype == DX_DTYPE_F16) return quantize_typed<__half>(p, sms, s);
-  return quantize_typed<__nv_bfloat16>(p, sms, s);
+  const bool vec = K % dx::kQuantVec == 0 && aligned16(X) && (ldx * elem_size(dtype)) % 16 == 0 &&
+                   aligned16(Q) && ldq % 8 == 0;
+  if (dtype == DX_DTYPE_F32)
+    return vec ? quantize_typed<float, true>(p, sms, s) : quantize_typed<float, false>(p, sms, s);
+  if (dtype == DX_DTYPE_F16)
+    return vec ? quantize_typed<__half, true>(p, sms, s) : quantize_typed<__half, false>(p, sms, s);
+  return vec ? quantize_typed<__nv_bfloat16, true>(p, sms, s)
+             : quantize_typed<__nv_bfloat16, false>(p, sms, s);
 }
 
 // --------------------------------------------------------------- problem

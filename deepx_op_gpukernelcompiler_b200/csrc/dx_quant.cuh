@@ -40,7 +40,6 @@ struct QuantParams {
   float* scale;
   int M, K;
   long long ldx, ldq;
-  int vec;  // X, Q and their pitches allow vector accesses
 };
 
 // One vector of 8 values as it lies in memory: 4 words of a 16-bit type, 8 of fp32.
@@ -50,11 +49,11 @@ struct QuantVec {
   uint32_t w[kWords];
 };
 
-// The vector at x, `n` values of it (zeros behind them).
-template <typename T>
-__device__ __forceinline__ QuantVec<T> quant_load(const T* x, int n, bool vec) {
+// The vector at x; kVec: aligned and whole, else `n` values of it (zeros behind them).
+template <bool kVec, typename T>
+__device__ __forceinline__ QuantVec<T> quant_load(const T* x, int n) {
   QuantVec<T> v;
-  if (vec && n >= kQuantVec) {
+  if constexpr (kVec) {
 #pragma unroll
     for (int i = 0; i < QuantVec<T>::kWords; i += 4) {
       const uint4 u = reinterpret_cast<const uint4*>(x)[i / 4];
@@ -130,8 +129,8 @@ __device__ __forceinline__ QuantRow quant_row(float top, bool finite) {
 }
 
 // The integers nearest to 127 x / a of a vector, stored as bytes.
-template <typename T>
-__device__ __forceinline__ void quant_store(int8_t* q, int n, bool vec, const QuantVec<T>& x,
+template <bool kVec, typename T>
+__device__ __forceinline__ void quant_store(int8_t* q, int n, const QuantVec<T>& x,
                                             const QuantRow& row) {
   constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the integer ends up in the low bits
   float f[kQuantVec];
@@ -169,7 +168,7 @@ __device__ __forceinline__ void quant_store(int8_t* q, int n, bool vec, const Qu
     b[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040),
                        __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
   if (row.c == 0.0f) b[0] = b[1] = 0u;  // a row with an infinity or a NaN
-  if (vec && n >= kQuantVec) {
+  if constexpr (kVec) {
     *reinterpret_cast<uint2*>(q) = make_uint2(b[0], b[1]);
   } else {
 #pragma unroll
@@ -180,66 +179,65 @@ __device__ __forceinline__ void quant_store(int8_t* q, int n, bool vec, const Qu
 
 // A row per CTA at a time, rows gridDim.x apart.  The next row's loads are issued
 // before this row's maximum is joined, so that they are in flight through the
-// barriers, the arithmetic and the stores.
-template <typename T, int THREADS>
+// barriers, the arithmetic and the stores.  kVec: every row consists of whole,
+// aligned vectors.
+template <typename T, int THREADS, bool kVec>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     quantize_rows_kernel(const QuantParams p) {
   constexpr int kWarps = THREADS / 32;
-  constexpr int kQuantRegs = kQuantRegsOf<T>;
+  constexpr int kRegs = kQuantRegsOf<T>;
   __shared__ uint32_t s_max[2][kWarps];
   grid_dependency_wait();
   grid_launch_dependents();
+  const int tid = static_cast<int>(threadIdx.x);
   const int vectors = (p.K + kQuantVec - 1) / kQuantVec;
-  const bool vec = p.vec != 0;
   const T* const X = static_cast<const T*>(p.X);
-  auto load_row = [&](long long row, QuantVec<T> (&f)[kQuantRegs]) {
+  auto load = [&](const T* x, int i) {
+    return quant_load<kVec>(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec);
+  };
+  auto load_row = [&](long long row, QuantVec<T> (&f)[kRegs]) {
+    const T* const x = X + row * p.ldx;
 #pragma unroll
-    for (int r = 0; r < kQuantRegs; ++r) {
-      const int i = r * THREADS + static_cast<int>(threadIdx.x);
-      if (i < vectors)
-        f[r] = quant_load(X + row * p.ldx + static_cast<long long>(i) * kQuantVec,
-                          p.K - i * kQuantVec, vec);
+    for (int r = 0; r < kRegs; ++r) {
+      const int i = r * THREADS + tid;
+      if (i < vectors) f[r] = load(x, i);
     }
   };
-  QuantVec<T> next[kQuantRegs];
+  QuantVec<T> next[kRegs];
   load_row(blockIdx.x, next);
   int half = 0;
   for (long long row = blockIdx.x; row < p.M; row += gridDim.x, half ^= 1) {
-    QuantVec<T> f[kQuantRegs];
+    QuantVec<T> f[kRegs];
     uint32_t m = 0;
 #pragma unroll
-    for (int r = 0; r < kQuantRegs; ++r) {
+    for (int r = 0; r < kRegs; ++r) {
       f[r] = next[r];
-      if (r * THREADS + static_cast<int>(threadIdx.x) < vectors) m = quant_max(m, f[r]);
+      if (r * THREADS + tid < vectors) m = quant_max(m, f[r]);
     }
     if (row + gridDim.x < p.M) load_row(row + gridDim.x, next);
     const T* const x = X + row * p.ldx;
     int8_t* const q = p.Q + row * p.ldq;
-    for (int i = kQuantRegs * THREADS + static_cast<int>(threadIdx.x); i < vectors; i += THREADS)
-      m = quant_max(m, quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec));
+    for (int i = kRegs * THREADS + tid; i < vectors; i += THREADS) m = quant_max(m, load(x, i));
     m = __reduce_max_sync(0xffffffffu, quant_max_bits<T>(m));
     // Two arrays in turn: a warp may be a row ahead of one still reading.
-    if ((threadIdx.x & 31) == 0) s_max[half][threadIdx.x >> 5] = m;
+    if ((tid & 31) == 0) s_max[half][tid >> 5] = m;
     __syncthreads();
-    m = s_max[half][0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) m = max(m, s_max[half][w]);
+    m = __reduce_max_sync(0xffffffffu, s_max[half][tid & (kWarps - 1)]);
 
     const bool finite = m < 0x7f800000u;
     const float top = fmaxf(__uint_as_float(finite ? m : 0u), 0x1p-100f);
-    if (threadIdx.x == 0)
+    if (tid == 0)
       p.scale[row] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
     const QuantRow qr = quant_row(top, finite);
 #pragma unroll
-    for (int r = 0; r < kQuantRegs; ++r) {
-      const int i = r * THREADS + static_cast<int>(threadIdx.x);
+    for (int r = 0; r < kRegs; ++r) {
+      const int i = r * THREADS + tid;
       if (i < vectors)
-        quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec, f[r], qr);
+        quant_store<kVec>(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, f[r], qr);
     }
-    for (int i = kQuantRegs * THREADS + static_cast<int>(threadIdx.x); i < vectors; i += THREADS)
-      quant_store(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec,
-                  quant_load(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, vec),
-                  qr);
+    for (int i = kRegs * THREADS + tid; i < vectors; i += THREADS)
+      quant_store<kVec>(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, load(x, i),
+                        qr);
   }
 }
 
