@@ -6,8 +6,8 @@
 //
 // Bound by memory: a row is read once into registers (rows of more than
 // the threads' registers hold are read twice, the second time from L2), its
-// largest magnitude found on the integer bit patterns (ordered as the
-// magnitudes are, and a NaN stays the largest), and one byte a value written.
+// largest magnitude found (a NaN counts as the largest), and one byte a value
+// written.
 //
 // The rounding is exact.  With c = 127 / a in fp32, x c is off by 2^-23 of the
 // quotient; one residual step, x c + (127 x - x c a) / a, leaves a half exactly a
@@ -49,8 +49,9 @@ struct QuantVec {
   uint32_t w[kWords];
 };
 
-// The vector at x; kVec: aligned and whole, else `n` values of it (zeros behind them).
-template <bool kVec, typename T>
+// Eight values: kVec: of the vector at x, else every kStride'th from x on, those
+// before `n` (zeros behind them).
+template <bool kVec, int kStride, typename T>
 __device__ __forceinline__ QuantVec<T> quant_load(const T* x, int n) {
   QuantVec<T> v;
   if constexpr (kVec) {
@@ -61,12 +62,13 @@ __device__ __forceinline__ QuantVec<T> quant_load(const T* x, int n) {
     }
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < kQuantVec; ++i) v.w[i] = i < n ? __float_as_uint(x[i]) : 0u;
+    for (int i = 0; i < kQuantVec; ++i) v.w[i] = i * kStride < n ? __float_as_uint(x[i * kStride]) : 0u;
   } else {
 #pragma unroll
     for (int i = 0; i < kQuantVec / 2; ++i) {
       const uint16_t* const u = reinterpret_cast<const uint16_t*>(x);
-      const uint32_t lo = 2 * i < n ? u[2 * i] : 0u, hi = 2 * i + 1 < n ? u[2 * i + 1] : 0u;
+      const uint32_t lo = 2 * i * kStride < n ? u[2 * i * kStride] : 0u;
+      const uint32_t hi = (2 * i + 1) * kStride < n ? u[(2 * i + 1) * kStride] : 0u;
       v.w[i] = lo | (hi << 16);
     }
   }
@@ -88,28 +90,38 @@ __device__ __forceinline__ void quant_floats(const QuantVec<T>& v, float (&f)[kQ
   }
 }
 
-// The larger of m and the magnitudes of the vector, as bit patterns of T: of
-// two 16-bit values at once, in both halves of m.  A NaN is the largest.
+// The larger of the magnitudes m (a pair of a 16-bit type, or one fp32) and w; a NaN
+// is the largest.
+__device__ __forceinline__ uint32_t quant_max_word(uint32_t m, uint32_t w, const __half*) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&m),
+                                __habs2(*reinterpret_cast<const __half2*>(&w)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t quant_max_word(uint32_t m, uint32_t w, const __nv_bfloat16*) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&m),
+                                       __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t quant_max_word(uint32_t m, uint32_t w, const float*) {
+  return max(m, w & 0x7fffffffu);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t quant_max(uint32_t m, const QuantVec<T>& v) {
 #pragma unroll
-  for (int i = 0; i < QuantVec<T>::kWords; ++i) {
-    if constexpr (sizeof(T) == 4)
-      m = max(m, v.w[i] & 0x7fffffffu);
-    else
-      m = __vmaxu2(m, v.w[i] & 0x7fff7fffu);
-  }
+  for (int i = 0; i < QuantVec<T>::kWords; ++i)
+    m = quant_max_word(m, v.w[i], static_cast<const T*>(nullptr));
   return m;
 }
 
-// The fp32 bit pattern of a quant_max.
+// A quant_max as the bit pattern of an fp32 magnitude (ordered as magnitudes are).
 template <typename T>
 __device__ __forceinline__ uint32_t quant_max_bits(uint32_t m) {
   if constexpr (sizeof(T) == 4) {
     return m;
   } else {
-    const float2 p = ElemTraits<T>::unpack2(max(m & 0xffffu, m >> 16));
-    return __float_as_uint(p.x) & 0x7fffffffu;
+    const float2 p = ElemTraits<T>::unpack2(m);
+    return max(__float_as_uint(p.x) & 0x7fffffffu, __float_as_uint(p.y) & 0x7fffffffu);
   }
 }
 
@@ -128,8 +140,9 @@ __device__ __forceinline__ QuantRow quant_row(float top, bool finite) {
   return r;
 }
 
-// The integers nearest to 127 x / a of a vector, stored as bytes.
-template <bool kVec, typename T>
+// The integers nearest to 127 x / a of eight values, stored as bytes where
+// quant_load found them.
+template <bool kVec, int kStride, typename T>
 __device__ __forceinline__ void quant_store(int8_t* q, int n, const QuantVec<T>& x,
                                             const QuantRow& row) {
   constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the integer ends up in the low bits
@@ -173,35 +186,36 @@ __device__ __forceinline__ void quant_store(int8_t* q, int n, const QuantVec<T>&
   } else {
 #pragma unroll
     for (int i = 0; i < kQuantVec; ++i)
-      if (i < n) q[i] = static_cast<int8_t>(b[i >> 2] >> (8 * (i & 3)));
+      if (i * kStride < n) q[i * kStride] = static_cast<int8_t>(b[i >> 2] >> (8 * (i & 3)));
   }
 }
 
 // A row per CTA at a time, rows gridDim.x apart.  The next row's loads are issued
 // before this row's maximum is joined, so that they are in flight through the
 // barriers, the arithmetic and the stores.  kVec: every row consists of whole,
-// aligned vectors.
+// aligned vectors, a thread taking every THREADS'th; else a thread takes every
+// THREADS'th value, so that a warp's loads and stores are contiguous all the same
+// (8192 x 4099 bf16: 67 us with eight neighbouring values a thread).
 template <typename T, int THREADS, bool kVec>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     quantize_rows_kernel(const QuantParams p) {
   constexpr int kWarps = THREADS / 32;
   constexpr int kRegs = kQuantRegsOf<T>;
+  constexpr int kBlock = THREADS * kQuantVec;  // values of a row that one step covers
   __shared__ uint32_t s_max[2][kWarps];
   grid_dependency_wait();
   grid_launch_dependents();
   const int tid = static_cast<int>(threadIdx.x);
-  const int vectors = (p.K + kQuantVec - 1) / kQuantVec;
-  const T* const X = static_cast<const T*>(p.X);
-  auto load = [&](const T* x, int i) {
-    return quant_load<kVec>(x + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec);
+  const int lead = kVec ? tid * kQuantVec : tid;  // this thread's first value of a step
+  const T* const X = static_cast<const T*>(p.X) + lead;
+  auto load = [&](const T* x, int at) {  // x: of the row, at `lead`; at: the step's first value
+    return quant_load<kVec, THREADS>(x + at, p.K - lead - at);
   };
   auto load_row = [&](long long row, QuantVec<T> (&f)[kRegs]) {
     const T* const x = X + row * p.ldx;
 #pragma unroll
-    for (int r = 0; r < kRegs; ++r) {
-      const int i = r * THREADS + tid;
-      if (i < vectors) f[r] = load(x, i);
-    }
+    for (int r = 0; r < kRegs; ++r)
+      if (r * kBlock + lead < p.K) f[r] = load(x, r * kBlock);
   };
   QuantVec<T> next[kRegs];
   load_row(blockIdx.x, next);
@@ -212,12 +226,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 #pragma unroll
     for (int r = 0; r < kRegs; ++r) {
       f[r] = next[r];
-      if (r * THREADS + tid < vectors) m = quant_max(m, f[r]);
+      if (r * kBlock + lead < p.K) m = quant_max(m, f[r]);
     }
     if (row + gridDim.x < p.M) load_row(row + gridDim.x, next);
     const T* const x = X + row * p.ldx;
-    int8_t* const q = p.Q + row * p.ldq;
-    for (int i = kRegs * THREADS + tid; i < vectors; i += THREADS) m = quant_max(m, load(x, i));
+    int8_t* const q = p.Q + row * p.ldq + lead;
+    for (int at = kRegs * kBlock; at + lead < p.K; at += kBlock) m = quant_max(m, load(x, at));
     m = __reduce_max_sync(0xffffffffu, quant_max_bits<T>(m));
     // Two arrays in turn: a warp may be a row ahead of one still reading.
     if ((tid & 31) == 0) s_max[half][tid >> 5] = m;
@@ -230,14 +244,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       p.scale[row] = finite ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
     const QuantRow qr = quant_row(top, finite);
 #pragma unroll
-    for (int r = 0; r < kRegs; ++r) {
-      const int i = r * THREADS + tid;
-      if (i < vectors)
-        quant_store<kVec>(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, f[r], qr);
-    }
-    for (int i = kRegs * THREADS + tid; i < vectors; i += THREADS)
-      quant_store<kVec>(q + static_cast<long long>(i) * kQuantVec, p.K - i * kQuantVec, load(x, i),
-                        qr);
+    for (int r = 0; r < kRegs; ++r)
+      if (r * kBlock + lead < p.K)
+        quant_store<kVec, THREADS>(q + r * kBlock, p.K - lead - r * kBlock, f[r], qr);
+    for (int at = kRegs * kBlock; at + lead < p.K; at += kBlock)
+      quant_store<kVec, THREADS>(q + at, p.K - lead - at, load(x, at), qr);
   }
 }
 
