@@ -3,7 +3,7 @@
 //   Y[m,n] = act(s_m tg_n sum_k Xq Wgq + bg[n]) * (s_m tu_n sum_k Xq Wuq + bu[n])
 // with Xq, Wq signed 8-bit, s (one per row of X: token) and t (one per output
 // channel) fp32, fp16 / bf16 / fp32 out.  The sums are exact: 32-bit integer
-// accumulators of tcgen05.mma kind::i8 (K <= 131072, so |sum| < 2^31 even where
+// accumulators of tcgen05.mma kind::i8 (K <= 131071, so |sum| < 2^31 even where
 // every product is 128 * 128); they become fp32 once, at the end.
 //
 // Both operands are K-major: rows of 128 bytes of K in 128-byte-swizzled
@@ -90,10 +90,15 @@ struct Int8TileShape {
   static constexpr int FULL_SM = 227 * 1024;
   // The partial sums received from a cluster of C CTAs, [source][row of this
   // CTA's share][128], lie in the idle ring: at most mn + C rows of 512 bytes.
-  static constexpr bool receive_fits(int mn, int stages) {
-    return (mn + MAX_CLUSTER) * 512 <= stages * stage_bytes(mn);
-  }
+  static constexpr int MIN_STAGES = 3;
+  static constexpr int half_sm_stages(int mn) { return (HALF_SM - smem_bytes(mn, 0)) / stage_bytes(mn); }
 };
+static_assert(Int8TileShape::half_sm_stages(Int8TileShape::MAX_MN) >= Int8TileShape::MIN_STAGES &&
+                  (16 + Int8TileShape::MAX_CLUSTER) * 512 <=
+                      Int8TileShape::MIN_STAGES * Int8TileShape::stage_bytes(16) &&
+                  (Int8TileShape::MAX_MN + Int8TileShape::MAX_CLUSTER) * 512 <=
+                      Int8TileShape::MIN_STAGES * Int8TileShape::stage_bytes(Int8TileShape::MAX_MN),
+              "receive area");
 
 // First row (of `rows`) of the share that CTA c of C finishes.
 __device__ __forceinline__ int int8_share(int c, int rows, int C) { return c * rows / C; }
@@ -257,6 +262,7 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
       }
     }
     done = mbar_wait(bar(S::BAR_TFULL), 0, abort_flag) && *abort_flag == 0;
+    done = __all_sync(0xffffffffu, done) != 0;  // (TMEM is read by whole warps)
     tc_fence_after();
     named_bar_sync(1, 128);  // s_sx
   }
@@ -714,7 +720,7 @@ __global__ void __launch_bounds__(Int8PairShape::THREADS, 1)
       // ahead (8192 x 14336 x 4096 with a residual: 363 us without).
       const bool ahead = p.tma_out && live > 0;
       if (ahead) epi_chunk_begin<S::EPI_BUFS>(c, n0, row_base, lane, it);
-      if (!mbar_wait(bar(S::BAR_TFULL + b), use_ph, abort_flag)) {
+      if (!mbar_wait_warp(bar(S::BAR_TFULL + b), use_ph, abort_flag)) {
         if (ahead) epi_chunk_drain<S::EPI_BUFS>(c, it);
         break;
       }

@@ -304,7 +304,7 @@ int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K,
  * dx_int8_workspace_size() bytes, which no other call may use meanwhile; it
  * needs no initial value).  bias, R and Y have type `dtype`; W is
  * 16-byte-aligned with ldw a multiple of 16.  The sums are exact (32-bit
- * integers, 1 <= K <= 131071) and become fp32 once.  `kernel` is
+ * integers, 1 <= K <= 131071; M <= 2^22, N <= 2^24) and become fp32 once.  `kernel` is
  * DX_KERNEL_AUTO, DX_KERNEL_UMMA (CTA pairs) or DX_KERNEL_DECODE (one tile per
  * CTA, K split over a cluster).  Outputs of the CTA pairs whose rows are 16-byte
  * aligned and 16-bit are stored by TMA; others go a row at a time.

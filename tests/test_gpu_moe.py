@@ -134,6 +134,14 @@ def test_strided_operands_untouched_rows_and_in_place():
     ref.check(got, ref.moe(**t, top_k=2, residual=t["X"]), "in place")
 
 
+@pytest.mark.parametrize("T,D,H,E,k", [(3, 40072, 72, 3, 2), (2, 136, 20000, 3, 2)])
+def test_whole_waves_of_tiles_in_either_phase(T, D, H, E, k):
+    """More 256-column tiles of the output, or 128-column tiles of h, than SMs."""
+    t = make(T, D, H, E, torch.bfloat16, bias=True, residual=True)
+    got = moe_ffn(**t, top_k=k, return_routing=True)
+    ref.check(got, ref.moe(**t, top_k=k))
+
+
 def test_one_expert_given_by_a_view():
     """E = 1: the expert pitch of a view plays no part."""
     t = make(3, 64, 40, 1, torch.bfloat16)
