@@ -42,6 +42,10 @@ using dx::UmmaShape;
 
 thread_local std::string t_last_error;
 thread_local std::string t_last_plan;
+// A plan of integers that dx_last_launch_plan formats when it is asked for: the
+// formatting is a noticeable part of a small call's host time.
+thread_local const char* t_plan_format = nullptr;
+thread_local int t_plan_ints[12];
 
 // Timeline buffer for the tensor-core kernels (dx_set_trace_buffer).
 std::atomic<unsigned long long*> g_trace{nullptr};
@@ -64,6 +68,15 @@ void set_plan(const char* fmt, ...) {
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
   t_last_plan = buf;
+  t_plan_format = nullptr;
+}
+
+template <typename... Ints>
+void set_plan_ints(const char* format, Ints... ints) {
+  static_assert(sizeof...(ints) <= 12, "plan integers");
+  t_plan_format = format;
+  int n = 0;
+  ((t_plan_ints[n++] = static_cast<int>(ints)), ...);
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
@@ -1359,7 +1372,17 @@ int dx_plan_destroy(dx_plan* plan) {
 
 const char* dx_last_error_string(void) { return t_last_error.c_str(); }
 
-const char* dx_last_launch_plan(void) { return t_last_plan.c_str(); }
+const char* dx_last_launch_plan(void) {
+  if (t_plan_format != nullptr) {
+    const int* const v = t_plan_ints;
+    char buf[256];
+    snprintf(buf, sizeof(buf), t_plan_format, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8],
+             v[9], v[10], v[11]);
+    t_last_plan = buf;
+    t_plan_format = nullptr;
+  }
+  return t_last_plan.c_str();
+}
 
 int dx_set_trace_buffer(void* device_buffer, size_t bytes) {
   t_last_error.clear();

@@ -246,9 +246,10 @@ int launch_int8_tile(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.w_early = pr.w_early ? 1 : 0;
   const int n_tiles = static_cast<int>((pr.N + NT - 1) / NT);
   const int m_tiles = static_cast<int>((pr.M + pl.mn - 1) / pl.mn);
-  set_plan("int8_tile%s tile=%dx%d stages=%d grid=%dx%d cluster=%d early=%d smem=%d",
-           G ? "_gated" : "", NT, pl.mn, pl.stages, n_tiles * pl.cluster, m_tiles, pl.cluster,
-           p.w_early, S::smem_bytes(pl.mn, pl.stages));
+  set_plan_ints(G ? "int8_tile_gated tile=%dx%d stages=%d grid=%dx%d cluster=%d early=%d smem=%d"
+                  : "int8_tile tile=%dx%d stages=%d grid=%dx%d cluster=%d early=%d smem=%d",
+                NT, pl.mn, pl.stages, n_tiles * pl.cluster, m_tiles, pl.cluster, p.w_early,
+                S::smem_bytes(pl.mn, pl.stages));
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = launch_config(n_tiles * pl.cluster, S::THREADS,
                                          S::smem_bytes(pl.mn, pl.stages), pr.stream, pl.cluster,
@@ -315,9 +316,10 @@ int launch_int8_pair(const Int8Problem& pr, int dev, const Int8Plan& pl) {
   p.num_work = p.full_tiles + 2 * (tiles - p.full_tiles);
   p.group_m = pick_group_m(p.m_tiles, 256, (pr.K + 1) / 2);
   p.workers = std::min(pl.workers, p.num_work);
-  set_plan("int8_pair%s tile=256x%d tma_out=%d stages=%d grid=%d tiles=%d full=%d group_m=%d smem=%d",
-           G ? "_gated" : "", NT, p.tma_out, p.stages, 2 * p.workers, tiles, p.full_tiles, p.group_m,
-           S::SMEM_BYTES);
+  set_plan_ints(
+      G ? "int8_pair_gated tile=256x%d tma_out=%d stages=%d grid=%d tiles=%d full=%d group_m=%d smem=%d"
+        : "int8_pair tile=256x%d tma_out=%d stages=%d grid=%d tiles=%d full=%d group_m=%d smem=%d",
+      NT, p.tma_out, p.stages, 2 * p.workers, tiles, p.full_tiles, p.group_m, S::SMEM_BYTES);
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg =
       launch_config(2 * p.workers, S::THREADS, S::SMEM_BYTES, pr.stream, 2, attr);

@@ -139,8 +139,7 @@ int launch_moe_experts(const dx_moe_args& a, int dev, int ctas, const MoeLayout&
                          CU_TENSOR_MAP_SWIZZLE_128B, "h")))
     return rc;
   const int smem = S::smem_bytes(mn, stages);
-  set_plan("moe T=%d mn=%d stages=%d grid=%d smem=%d workspace=%zu", p.T, mn, stages, ctas, smem,
-           l.bytes);
+  set_plan_ints("moe T=%d mn=%d stages=%d grid=%d smem=%d", p.T, mn, stages, ctas, smem);
   // Cooperative: the CTAs wait for one another, so all of them or none are placed.
   cudaLaunchAttribute attr[3];
   cudaLaunchConfig_t cfg = launch_config(ctas, S::THREADS, smem, stream, 1, attr);

@@ -177,7 +177,8 @@ def _output(name: str, out, x: torch.Tensor, M: int, N: int, dtype: torch.dtype)
     if not x.is_cuda:
         raise ValueError(f"{name} runs on CUDA tensors only (the engine has no CPU path)")
     if out is None:
-        return x.new_empty((M, N), dtype=dtype), max(N, 1)
+        new = x.new_empty((M, N)) if x.dtype is dtype else x.new_empty((M, N), dtype=dtype)
+        return new, max(N, 1)
     _check_matrix("out", out, M, N)
     _like("out", out, x, dtype)
     return out, _ld(out)
@@ -208,17 +209,6 @@ def _on_device(index: int, call):
         return call(_raw_stream(index))
 
 
-def _workspace(lib, x: torch.Tensor, x_scale, M: int, K: int):
-    # Of this call alone, from the allocator of the current stream or of the
-    # graph being captured: calls on other streams and other graphs cannot share
-    # it, and the allocator keeps it from others until the launches are done.
-    if x_scale is not None or M == 0:
-        return None, None, 0
-    size = lib.dx_int8_workspace_size(M, K)
-    space = x.new_empty(size, dtype=torch.uint8)
-    return space, space.data_ptr(), size
-
-
 def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
                 residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
                 dtype: torch.dtype | None = None, kernel: str = "auto") -> torch.Tensor:
@@ -243,11 +233,20 @@ def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
     lib = nat.load()
 
     def call(stream):
-        space, ws_ptr, ws_bytes = _workspace(lib, x, x_scale, M, K)
+        # The workspace is this call's alone, from the allocator of the current
+        # stream or of the graph being captured: calls on other streams and other
+        # graphs cannot share it, and it stays theirs until the launches are done.
+        ws_ptr, ws_bytes, sx_ptr = None, 0, None
+        if x_scale is not None:
+            sx_ptr = x_scale.data_ptr()
+        elif M:
+            ws_bytes = lib.dx_int8_workspace_size(M, K)
+            space = x.new_empty(ws_bytes, dtype=torch.uint8)
+            ws_ptr = space.data_ptr()
         return lib.dx_int8_linear(
-            x.data_ptr(), x_code, x_scale.data_ptr() if x_scale is not None else None,
-            wq.data_ptr(), ws.data_ptr(), b_ptr, r_ptr, out.data_ptr(), M, N, K, ldx, ldw, ldr,
-            ldy, DTYPE_CODES[dtype], act, kcode, ws_ptr, ws_bytes, stream)
+            x.data_ptr(), x_code, sx_ptr, wq.data_ptr(), ws.data_ptr(), b_ptr, r_ptr,
+            out.data_ptr(), M, N, K, ldx, ldw, ldr, ldy, DTYPE_CODES[dtype], act, kcode, ws_ptr,
+            ws_bytes, stream)
 
     rc = _on_device(index, call)
     if rc:
@@ -273,12 +272,17 @@ def int8_gated_linear(X, Wg, Wu, bias_g: torch.Tensor | None = None,
     lib = nat.load()
 
     def call(stream):
-        space, ws_ptr, ws_bytes = _workspace(lib, x, x_scale, M, K)
+        ws_ptr, ws_bytes, sx_ptr = None, 0, None  # as in int8_linear
+        if x_scale is not None:
+            sx_ptr = x_scale.data_ptr()
+        elif M:
+            ws_bytes = lib.dx_int8_workspace_size(M, K)
+            space = x.new_empty(ws_bytes, dtype=torch.uint8)
+            ws_ptr = space.data_ptr()
         return lib.dx_int8_gated_linear(
-            x.data_ptr(), x_code, x_scale.data_ptr() if x_scale is not None else None,
-            gq.data_ptr(), gs.data_ptr(), uq.data_ptr(), us.data_ptr(), bg_ptr, bu_ptr,
-            out.data_ptr(), M, N, K, ldx, ldg, ldu, ldy, DTYPE_CODES[dtype], act, kcode, ws_ptr,
-            ws_bytes, stream)
+            x.data_ptr(), x_code, sx_ptr, gq.data_ptr(), gs.data_ptr(), uq.data_ptr(),
+            us.data_ptr(), bg_ptr, bu_ptr, out.data_ptr(), M, N, K, ldx, ldg, ldu, ldy,
+            DTYPE_CODES[dtype], act, kcode, ws_ptr, ws_bytes, stream)
 
     rc = _on_device(index, call)
     if rc:
