@@ -95,7 +95,8 @@ int launch_moe_experts(const dx_moe_args& a, int dev, int ctas, const MoeLayout&
   using S = MoeShape;
   auto kern = dx::moe_experts_kernel<MN, T>;
   const int mn = static_cast<int>((a.T + 15) / 16 * 16);
-  const int stages = S::max_stages(mn);
+  const int pairs = static_cast<int>(a.T * a.top_k);
+  const int stages = S::max_stages(mn, pairs);
   int rc = ensure_smem_attr(dev, reinterpret_cast<const void*>(kern), 227 * 1024, true);
   if (rc) return rc;
   char* const ws = static_cast<char*>(a.workspace);
@@ -138,7 +139,7 @@ int launch_moe_experts(const dx_moe_args& a, int dev, int ctas, const MoeLayout&
   if ((rc = make_tmap_2d(&tLo, p.h_lo, dt, a.H, l.chosen * a.T, a.H, 64, mn,
                          CU_TENSOR_MAP_SWIZZLE_128B, "h")))
     return rc;
-  const int smem = S::smem_bytes(mn, stages);
+  const int smem = S::smem_bytes(mn, stages, pairs);
   set_plan_ints("moe T=%d mn=%d stages=%d grid=%d smem=%d", p.T, mn, stages, ctas, smem);
   // Cooperative: the CTAs wait for one another, so all of them or none are placed.
   cudaLaunchAttribute attr[3];
