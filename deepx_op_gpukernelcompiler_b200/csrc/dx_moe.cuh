@@ -30,6 +30,10 @@
 //     Between the phases the CTAs wait for one another, with the first weights
 //     of phase 2 already on their way.
 //
+// Both launches (us, weights from HBM; the chosen experts' bytes at the measured copy
+// rate): 1 token, 2 of 8 experts of 4096 x 14336 122 (108); 8 tokens, 8 of 64 of 2048 x
+// 1024 99 (81); 64 tokens of the same 150 (123); 33 tokens, 4 of 16 of 1032 x 2824 75 (43).
+//
 // Every wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once
 
@@ -43,7 +47,6 @@ namespace dx {
 constexpr int kMoeMaxT = 64;
 constexpr int kMoeMaxE = 256;
 constexpr int kMoeMaxTop = 32;
-constexpr int kMoeWholeBlocks = 10;
 
 // ---------------------------------------------------------------- router
 constexpr int kRouterThreads = 1024;
@@ -277,18 +280,15 @@ struct MoeRun {
 // 8 tokens, 64 experts of 2048 x 1024: 336 tiles on 148 CTAs).
 struct MoePhase {
   int tiles, whole, per_tile;  // tiles [0, whole) are whole; units of a tile
-  int units, ctas;             // of the split tiles; CTAs that have some
+  int each, more;              // split units of a CTA; the first `more` CTAs have one more
   int nt, kb;                  // phase 1: tiles of an expert; K blocks of an expert's product
   int u0, u1;                  // this CTA's units
   bool second;
 
-  __device__ __forceinline__ int begin(int g) const {
-    return static_cast<int>(static_cast<long long>(g) * units / ctas);
-  }
+  __device__ __forceinline__ int begin(int g) const { return g * each + min(g, more); }
   __device__ __forceinline__ int cta_of(int u) const {
-    int g = static_cast<int>(static_cast<long long>(u) * ctas / units);
-    while (g + 1 < ctas && begin(g + 1) <= u) ++g;
-    return g;
+    const int front = more * (each + 1);
+    return u < front ? u / (each + 1) : more + (u - front) / each;
   }
   // The work item at position i of this CTA's list (its units, then the units of
   // its whole tiles): tile, expert index and K block.
@@ -337,22 +337,29 @@ __device__ __forceinline__ MoePhase moe_phase(const MoeParams& p, int chosen, bo
   f.per_tile = second ? chosen * p.kb_h : p.kb_d;
   f.tiles = second ? p.nt_d : chosen * p.nt_h;
   f.whole = f.tiles / grid * grid;
-  // Fewer tiles than CTAs, and short ones: joining partial sums (some 5 us) costs more
-  // than the K blocks it saves the CTAs that have a tile (some 0.5 us each).
-  if (!second && f.whole == 0 && f.per_tile - f.tiles * f.per_tile / grid <= kMoeWholeBlocks)
-    f.whole = f.tiles;
-  f.units = (f.tiles - f.whole) * f.per_tile;
-  f.ctas = min(grid, f.units);  // (0: no split tiles)
-  f.u0 = g < f.ctas ? f.begin(g) : 0;
-  f.u1 = g < f.ctas ? f.begin(g + 1) : 0;
+  const int units = (f.tiles - f.whole) * f.per_tile;
+  f.each = units / grid;
+  f.more = units - f.each * grid;
+  f.u0 = f.begin(g);
+  f.u1 = f.begin(g + 1);
   return f;
+}
+
+// Counts a CTA in: what it wrote before, and what threads wrote that it met at a barrier
+// since, is seen by whoever sees the count.  (One release for the CTA: a fence by each
+// of 128 threads takes some 2 us.)
+__device__ __forceinline__ void moe_arrive(int* ctr) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(ctr) : "memory");
 }
 
 // Bounded wait until *ctr reaches `target` (every CTA of the launch is resident).
 __device__ __forceinline__ bool moe_wait(const int* ctr, int target, volatile int* abort_flag) {
   const uint64_t t0 = global_timer_ns();
   uint32_t spins = 0;
-  while (*reinterpret_cast<const volatile int*>(ctr) < target) {
+  while (true) {
+    int n;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(n) : "l"(ctr) : "memory");
+    if (n >= target) return true;
     __nanosleep(20);
     if ((++spins & 63u) == 0) {
       if (*abort_flag) return false;
@@ -363,8 +370,18 @@ __device__ __forceinline__ bool moe_wait(const int* ctr, int target, volatile in
       }
     }
   }
-  __threadfence();
-  return true;
+}
+
+// A store under a predicate, and no branch: a thread makes up to 128 of them in a row.
+// With a branch around each, a call took 1 to 3 us longer (its code comes from memory
+// about once a call, as the weights leave none of it in L2).
+__device__ __forceinline__ void moe_store_if(float* at, float v, uint32_t c) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "@p st.global.f32 [%0], %1;\n\t}" ::"l"(at),
+      "f"(v), "r"(c)
+      : "memory");
 }
 
 // h as hi + lo of type T.
@@ -670,13 +687,11 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         if (first != g) slot = f.begin(first) / f.per_tile == tile - f.whole ? 0 : 1;
       }
       sum = part(first, slot);
-      __threadfence();
       named_bar_sync(1, 128);
-      if (whole) return true;
       if (et == 0) {
         int* const ctr = p.counters + (f.second ? gridDim.x : 0) + first;
-        atomicAdd(ctr, 1);
-        *s_ok = share < 0 || moe_wait(ctr, peers, abort_flag) ? 1 : 0;
+        if (!whole) moe_arrive(ctr);
+        *s_ok = whole || share < 0 || moe_wait(ctr, peers, abort_flag) ? 1 : 0;
       }
       named_bar_sync(1, 128);  // (behind it the partials are read from L2, past L1)
       return *s_ok != 0;
@@ -747,11 +762,10 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
             float* const to = part(g, slot) + mc * 128 + n;
             float* const to1 = to + p.T * 128;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if ((some >> j) & 1u) {
-                to[j * 128] = __uint_as_float(a0[j]);
-                to1[j * 128] = __uint_as_float(a1[j]);
-              }
+            for (int j = 0; j < 16; ++j) {
+              moe_store_if(to + j * 128, __uint_as_float(a0[j]), (some >> j) & 1u);
+              moe_store_if(to1 + j * 128, __uint_as_float(a1[j]), (some >> j) & 1u);
+            }
           } else {
             float v[16];
 #pragma unroll
@@ -772,11 +786,19 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(S::BAR_TEMPTY + b));
         if (whole) continue;
+        // (loaded before the wait for the other CTAs' sums)
+        const int col = col0 + 4 * lane;
+        float vg4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, vu4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (col < p.H) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            vg4[k] = moe_bias(bg, static_cast<long long>(e) * p.H + col + k);
+            vu4[k] = moe_bias(bu, static_cast<long long>(e) * p.H + col + k);
+          }
+        }
         ok = join(f, r.tile, slot, false);
         if (!ok || share < 0) continue;
         // This CTA's share of the tokens, a warp each; a lane has four columns.
-        const int col = col0 + 4 * lane;
-        const long long bi = static_cast<long long>(e) * p.H + col;
         int i = 0;
 #pragma unroll 1
         for (unsigned long long left = mask; left != 0; left &= left - 1, ++i) {
@@ -788,8 +810,8 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
           float v[4] = {t[0].x, t[0].y, t[0].z, t[0].w}, w[4] = {t[1].x, t[1].y, t[1].z, t[1].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            v[k] += moe_bias(bg, bi + k);
-            w[k] += moe_bias(bu, bi + k);
+            v[k] += vg4[k];
+            w[k] += vu4[k];
           }
           act_values<false>(v, p.act);
           __align__(8) T hi[4];
@@ -802,11 +824,10 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         }
       }
     }
-    // Everything this CTA wrote of h, before any CTA reads it by TMA.
-    fence_proxy_async_global();
-    __threadfence();
+    // Everything this CTA wrote of h, before any CTA reads it by TMA (the proxies'
+    // fence is the reader's, behind its wait).
     named_bar_sync(1, 128);
-    if (et == 0 && ok) atomicAdd(barrier_ctr, 1);
+    if (et == 0 && ok) moe_arrive(barrier_ctr);
 
     {  // ---- phase 2: the output
       const MoePhase f = moe_phase(p, chosen, true);
@@ -826,8 +847,11 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         float* const roww = s_roww + b * kMoeMaxT;
         if (et < p.T) {
           float w = 0.0f;
-          for (int j = 0; j < p.top; ++j)
-            if (s_ids[et * p.top + j] == e) w = s_wts[et * p.top + j];
+#pragma unroll 4
+          for (int j = 0; j < p.top; ++j) {
+            const float wj = s_wts[et * p.top + j];
+            w = s_ids[et * p.top + j] == e ? wj : w;
+          }
           roww[et] = w;
         }
         float vb[2] = {0.0f, 0.0f};
@@ -847,15 +871,20 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         for (int mc = 0; mc < MN; mc += 16) {
           const uint32_t some = static_cast<uint32_t>(mask >> mc) & 0xffffu;
           if (some != 0) {
+            float w[16];
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(w + j) = *reinterpret_cast<const float4*>(roww + mc + j);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t v[16];
               tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(h * MN + mc), v);
               tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if ((some >> j) & 1u)
-                  y[h][mc + j] = fmaf(roww[mc + j], __uint_as_float(v[j]) + vb[h], y[h][mc + j]);
+              for (int j = 0; j < 16; ++j) {
+                const float sum = fmaf(w[j], __uint_as_float(v[j]) + vb[h], y[h][mc + j]);
+                y[h][mc + j] = ((some >> j) & 1u) != 0 ? sum : y[h][mc + j];
+              }
             }
           }
         }
@@ -872,10 +901,8 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         float* const to1 = to + p.T * 128;
 #pragma unroll
         for (int m = 0; m < MN; ++m) {
-          if (m < p.T) {
-            to[m * 128] = y[0][m];
-            to1[m * 128] = y[1][m];
-          }
+          moe_store_if(to + m * 128, y[0][m], m < p.T);
+          moe_store_if(to1 + m * 128, y[1][m], m < p.T);
           y[0][m] = y[1][m] = 0.0f;
         }
         ok = join(f, r.tile, slot, whole);
@@ -883,17 +910,19 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         // This CTA's share of the rows (halves of a token's 256 columns), a warp each.
 #pragma unroll 1
         for (int row = share * 4 + q; row < 2 * p.T; row += 4 * shares) {
-          float4 t;
-          row_sums(std::integral_constant<int, 1>(), row, 0, &t);
           const int h = row >= p.T ? 1 : 0, m = row - h * p.T;
           const int c = r.tile * 256 + 128 * h + 4 * lane;
-          if (c >= p.D) continue;
-          float v[4] = {t.x, t.y, t.z, t.w};
+          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (res != nullptr && c < p.D) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (res != nullptr) v[k] += Tr::to_float(res[m * p.ldr + c + k]);
-            Y[m * p.ldy + c + k] = Tr::from_float(v[k]);
+            for (int k = 0; k < 4; ++k) v[k] = Tr::to_float(res[m * p.ldr + c + k]);
           }
+          float4 t;
+          row_sums(std::integral_constant<int, 1>(), row, 0, &t);
+          if (c >= p.D) continue;
+          const float s[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) Y[m * p.ldy + c + k] = Tr::from_float(s[k] + v[k]);
         }
       }
     }
