@@ -75,7 +75,8 @@ struct Int8TileShape {
   static constexpr int MAX_CLUSTER = 8;
   static constexpr int THREADS = 192;
   // Shared memory: the ring of `stages` W tiles, then as many X tiles, then
-  static constexpr int OFF_BAR = MAX_MN * 4;  // (behind MAX_MN row scales)
+  static constexpr int OFF_DEST = MAX_MN * 4;  // (behind MAX_MN row scales)
+  static constexpr int OFF_BAR = OFF_DEST + MAX_MN * 4;
   static constexpr int BAR_FULL = 0;
   static constexpr int BAR_EMPTY = MAX_STAGES;
   static constexpr int BAR_TFULL = 2 * MAX_STAGES;
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
   const uint32_t tail = static_cast<uint32_t>(stages) * stage_bytes;
   const uint32_t bars = base + tail + S::OFF_BAR;
   float* const s_sx = reinterpret_cast<float*>(base_ptr + tail);
+  uint32_t* const s_dest = reinterpret_cast<uint32_t*>(base_ptr + tail + S::OFF_DEST);
   uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(base_ptr + tail + S::OFF_MISC);
   volatile int* const abort_flag =
       reinterpret_cast<volatile int*>(base_ptr + tail + S::OFF_MISC + 4);
@@ -197,6 +199,10 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
   const int nt = kGated ? (et & 63) : (via_smem ? et : q * 32 + lane);
   const int ncol = nt < p.nr ? n0 + nt : p.N;  // (p.N: none)
   float t0 = 0.0f, t1 = 0.0f, b0 = 0.0f, b1 = 0.0f;
+  // The rows this CTA finishes, this thread's first one and its residual.
+  const int my_row0 = int8_share(c, rows, C), my_rows = int8_share(c + 1, rows, C) - my_row0;
+  const int my_first = kGated ? (et >> 6) & 1 : 0;
+  float res0 = 0.0f;
 
   if (warp == 0) {
     // ------------------------------------------------------ TMA producer
@@ -252,7 +258,18 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
     __syncwarp();
   } else {
     // --------------------------------------------------------- epilogue
-    if (et < rows) s_sx[et] = p.sx[m0 + et];
+    if (et < rows) {
+      s_sx[et] = p.sx[m0 + et];
+      if (via_smem) {
+        // Where this CTA's partial sums of row et go: the CTA whose share has the row.
+        // (Found row by row behind the wait, 16 rows of 4096 x 4096 took 10.3 us, now 8.8.)
+        const int dest = ((et + 1) * C - 1) / rows;
+        const int first = int8_share(dest, rows, C);
+        const int share = int8_share(dest + 1, rows, C) - first;
+        const uint32_t at = base + static_cast<uint32_t>((c * share + et - first) * 512);
+        s_dest[et] = mapa_shared(at, static_cast<uint32_t>(dest));
+      }
+    }
     if (ncol < p.N) {
       t0 = p.sw[ncol];
       if (p.bias != nullptr) b0 = ld_elem(p.bias, ncol, static_cast<const T*>(nullptr));
@@ -261,6 +278,9 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
         if (p.bias2 != nullptr) b1 = ld_elem(p.bias2, ncol, static_cast<const T*>(nullptr));
       }
     }
+    if (via_smem && p.residual != nullptr && ncol < p.N && my_first < my_rows)
+      res0 = ld_elem(p.residual, (m0 + my_row0 + my_first) * p.ldr + ncol,
+                     static_cast<const T*>(nullptr));
     done = mbar_wait(bar(S::BAR_TFULL), 0, abort_flag) && *abort_flag == 0;
     done = __all_sync(0xffffffffu, done) != 0;  // (TMEM is read by whole warps)
     tc_fence_after();
@@ -275,26 +295,19 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
     else
       __syncthreads();
     if (warp >= 2 && done) {
-      int dest = 0, end = int8_share(1, rows, C), first = 0;
+      const uint32_t mine = static_cast<uint32_t>((q * 32 + lane) * 4);
 #pragma unroll 1
       for (int mc = 0; mc < rows; mc += 16) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(lane_addr + static_cast<uint32_t>(mc), r);
+        uint32_t to[16];  // (behind the last row: not used)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          *reinterpret_cast<uint4*>(to + j) = *reinterpret_cast<const uint4*>(s_dest + mc + j);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int m = mc + j;
-          if (m < rows) {
-            while (m >= end) {  // at most C steps in all
-              ++dest;
-              first = end;
-              end = int8_share(dest + 1, rows, C);
-            }
-            const uint32_t off =
-                static_cast<uint32_t>(((c * (end - first) + m - first) * 128 + q * 32 + lane) * 4);
-            st_shared_cluster_u32(mapa_shared(base + off, static_cast<uint32_t>(dest)), r[j]);
-          }
-        }
+        for (int j = 0; j < 16; ++j)
+          if (mc + j < rows) st_shared_cluster_u32(to[j] + mine, r[j]);
       }
     }
     tc_fence_before();
@@ -304,26 +317,29 @@ __global__ void __launch_bounds__(Int8TileShape::THREADS, 2)
       __syncthreads();
     if (warp >= 2 && done && ncol < p.N) {
       const int* const recv = reinterpret_cast<const int*>(base_ptr);
-      const int r0 = int8_share(c, rows, C), nr = int8_share(c + 1, rows, C) - r0;
       constexpr int kStep = kGated ? 2 : 1;
-      for (int i = kGated ? et >> 6 : 0; i < nr; i += kStep) {
-        const long long m = m0 + r0 + i;
+      float res = res0;
+#pragma unroll 1
+      for (int i = my_first; i < my_rows; i += kStep) {
+        const long long m = m0 + my_row0 + i;
+        float next = 0.0f;
+        if (p.residual != nullptr && i + kStep < my_rows)
+          next = ld_elem(p.residual, (m + kStep) * p.ldr + ncol, static_cast<const T*>(nullptr));
         int a0 = 0, a1 = 0;
 #pragma unroll
         for (int s = 0; s < S::MAX_CLUSTER; ++s) {
           if (s < C) {
-            const int* const src = recv + (s * nr + i) * 128 + (kGated ? (et & 63) : et);
+            const int* const src = recv + (s * my_rows + i) * 128 + (kGated ? (et & 63) : et);
             a0 += src[0];
             if (kGated) a1 += src[64];
           }
         }
-        const float sx = s_sx[r0 + i];
+        const float sx = s_sx[my_row0 + i];
         float v[1] = {fmaf(static_cast<float>(a0), sx * t0, b0)};
         act_values<sizeof(T) == 4>(v, p.act);
         if (kGated) v[0] *= fmaf(static_cast<float>(a1), sx * t1, b1);
-        if (p.residual != nullptr)
-          v[0] += ld_elem(p.residual, m * p.ldr + ncol, static_cast<const T*>(nullptr));
-        Y[m * p.ldy + ncol] = Tr::from_float(v[0]);
+        Y[m * p.ldy + ncol] = Tr::from_float(v[0] + res);
+        res = next;
       }
     }
   } else if (warp >= 2 && done) {

@@ -47,6 +47,7 @@ namespace dx {
 constexpr int kMoeMaxT = 64;
 constexpr int kMoeMaxE = 256;
 constexpr int kMoeMaxTop = 32;
+constexpr int kMoeWholeBlocks = 10;
 
 // ---------------------------------------------------------------- router
 constexpr int kRouterThreads = 1024;
@@ -337,6 +338,11 @@ __device__ __forceinline__ MoePhase moe_phase(const MoeParams& p, int chosen, bo
   f.per_tile = second ? chosen * p.kb_h : p.kb_d;
   f.tiles = second ? p.nt_d : chosen * p.nt_h;
   f.whole = f.tiles / grid * grid;
+  // Fewer tiles than CTAs, and short ones: joining partial sums costs more than the K
+  // blocks it saves the CTAs that have a tile (20 tokens, 2 of 60 experts of 1024 x 512:
+  // 32.4 us whole, 35.1 split; 1 token, 1 of 8 of 2048 x 4096: 42.6 and 27.1).
+  if (!second && f.whole == 0 && f.per_tile - f.tiles * f.per_tile / grid <= kMoeWholeBlocks)
+    f.whole = f.tiles;
   const int units = (f.tiles - f.whole) * f.per_tile;
   f.each = units / grid;
   f.more = units - f.each * grid;
@@ -370,18 +376,6 @@ __device__ __forceinline__ bool moe_wait(const int* ctr, int target, volatile in
       }
     }
   }
-}
-
-// A store under a predicate, and no branch: a thread makes up to 128 of them in a row.
-// With a branch around each, a call took 1 to 3 us longer (its code comes from memory
-// about once a call, as the weights leave none of it in L2).
-__device__ __forceinline__ void moe_store_if(float* at, float v, uint32_t c) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.u32 p, %2, 0;\n\t"
-      "@p st.global.f32 [%0], %1;\n\t}" ::"l"(at),
-      "f"(v), "r"(c)
-      : "memory");
 }
 
 // h as hi + lo of type T.
@@ -762,10 +756,11 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
             float* const to = part(g, slot) + mc * 128 + n;
             float* const to1 = to + p.T * 128;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              moe_store_if(to + j * 128, __uint_as_float(a0[j]), (some >> j) & 1u);
-              moe_store_if(to1 + j * 128, __uint_as_float(a1[j]), (some >> j) & 1u);
-            }
+            for (int j = 0; j < 16; ++j)
+              if ((some >> j) & 1u) {
+                to[j * 128] = __uint_as_float(a0[j]);
+                to1[j * 128] = __uint_as_float(a1[j]);
+              }
           } else {
             float v[16];
 #pragma unroll
@@ -881,7 +876,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
               tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(h * MN + mc), v);
               tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
+              for (int j = 0; j < 16; ++j) {  // (a branch a token: 64 tokens 1 us longer)
                 const float sum = fmaf(w[j], __uint_as_float(v[j]) + vb[h], y[h][mc + j]);
                 y[h][mc + j] = ((some >> j) & 1u) != 0 ? sum : y[h][mc + j];
               }
@@ -901,8 +896,10 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         float* const to1 = to + p.T * 128;
 #pragma unroll
         for (int m = 0; m < MN; ++m) {
-          moe_store_if(to + m * 128, y[0][m], m < p.T);
-          moe_store_if(to1 + m * 128, y[1][m], m < p.T);
+          if (m < p.T) {
+            to[m * 128] = y[0][m];
+            to1[m * 128] = y[1][m];
+          }
           y[0][m] = y[1][m] = 0.0f;
         }
         ok = join(f, r.tile, slot, whole);
