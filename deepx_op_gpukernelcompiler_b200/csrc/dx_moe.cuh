@@ -37,6 +37,7 @@
 // Every wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "dx_epilogue.cuh"
@@ -50,9 +51,18 @@ constexpr int kMoeMaxTop = 32;
 constexpr int kMoeWholeBlocks = 10;
 
 // ---------------------------------------------------------------- router
-constexpr int kRouterThreads = 1024;
 constexpr int kRouterTokens = 8;  // tokens of a cluster = its CTAs
 constexpr int kRouterRows = 512;  // rows of Wr per step, at most
+constexpr int kRouterBatch = 16;  // rows of Wr a thread, per step
+// Threads of a CTA: 1024, or 512 where those read their share of Wr in one step as well
+// (a call 1.0 to 1.4 us shorter, of 17 to 48: half as many sums to add; 0.3 to 1.1 us
+// longer where it takes them a second step).
+constexpr int router_threads(int D, int E) {
+  return (D + kRouterTokens - 1) / kRouterTokens <=
+                 std::min(kRouterRows, kRouterBatch * (512 / ((E + 31) / 32 * 32)))
+             ? 512
+             : 1024;
+}
 
 struct MoeRouterParams {
   const void* X;
@@ -72,11 +82,11 @@ __device__ __forceinline__ uint32_t moe_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRouterParams p) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) moe_router_kernel(const MoeRouterParams p) {
   using Tr = ElemTraits<T>;
-  __shared__ __align__(16) float s_x[kRouterThreads][kRouterTokens];  // [row][token]
-  static_assert(kRouterRows <= kRouterThreads, "a step's rows");
+  __shared__ __align__(16) float s_x[THREADS][kRouterTokens];  // [row][token]
+  static_assert(kRouterRows <= THREADS, "a step's rows");
   float* const s_part = &s_x[0][0];  // [row group][token][expert], once s_x is done with
   __shared__ float s_sum[kRouterTokens][kMoeMaxE];
   __shared__ float s_logit[kMoeMaxE];
@@ -87,20 +97,20 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRou
   grid_dependency_wait();
   grid_launch_dependents();
   if (blockIdx.x == 0)
-    for (int i = tid; i < p.num_counters; i += kRouterThreads) p.counters[i] = 0;
+    for (int i = tid; i < p.num_counters; i += THREADS) p.counters[i] = 0;
 
   // Threads as row groups x experts; each sums its rows for all tokens.  Wr's rows
   // are asked for before the tokens' values are needed: one trip to memory a step.
   const int ep = (p.E + 31) / 32 * 32;
-  const int groups = kRouterThreads / ep;
+  const int groups = THREADS / ep;
   const int e = tid % ep, kg = tid / ep;
   const bool live = kg < groups && e < p.E;
   const int slice = (p.D + kRouterTokens - 1) / kRouterTokens;
   const int k_begin = rank * slice, k_end = min(p.D, k_begin + slice);
   const T* const X = static_cast<const T*>(p.X);
   const T* const Wr = static_cast<const T*>(p.Wr);
-  constexpr int kBatch = 16;                                            // rows of Wr a thread, per step
-  constexpr int kPerThread = kRouterRows * kRouterTokens / kRouterThreads;  // token values
+  constexpr int kBatch = kRouterBatch;
+  constexpr int kPerThread = kRouterRows * kRouterTokens / THREADS;  // token values
   const int step = min(kRouterRows, kBatch * groups);  // rows of Wr per step
   float acc[kRouterTokens];
 #pragma unroll
@@ -110,7 +120,7 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRou
     T w[kBatch], x[kPerThread];
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      const int at = i * kRouterThreads + tid, t = at / kRouterRows, k = at % kRouterRows;
+      const int at = i * THREADS + tid, t = at / kRouterRows, k = at % kRouterRows;
       x[i] = t < tokens && k < rows ? X[(t0 + t) * p.ldx + k0 + k] : Tr::from_float(0.0f);
     }
 #pragma unroll
@@ -121,7 +131,7 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRou
     if (k0 != k_begin) __syncthreads();  // the previous step's values are no longer read
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      const int at = i * kRouterThreads + tid;
+      const int at = i * THREADS + tid;
       s_x[at % kRouterRows][at / kRouterRows] = Tr::to_float(x[i]);
     }
     __syncthreads();
@@ -151,7 +161,7 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRou
     for (int t = 0; t < kRouterTokens; ++t) s_part[(kg * kRouterTokens + t) * ep + e] = acc[t];
   }
   __syncthreads();
-  for (int i = tid; i < kRouterTokens * ep; i += kRouterThreads) {
+  for (int i = tid; i < kRouterTokens * ep; i += THREADS) {
     const int t = i / ep, ee = i % ep;
     float s = 0.0f;
     for (int g = 0; g < groups; ++g) s += s_part[(g * kRouterTokens + t) * ep + ee];
@@ -160,7 +170,7 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRou
   cluster_sync();
   const int token = t0 + rank;
   if (rank < tokens) {
-    for (int i = tid; i < p.E; i += kRouterThreads) {
+    for (int i = tid; i < p.E; i += THREADS) {
       float s = 0.0f;
 #pragma unroll
       for (int c = 0; c < kRouterTokens; ++c)

@@ -142,6 +142,15 @@ def test_whole_waves_of_tiles_in_either_phase(T, D, H, E, k):
     ref.check(got, ref.moe(**t, top_k=k))
 
 
+@pytest.mark.parametrize("D,E", [(1024, 64), (1032, 64), (256, 200), (264, 200), (4096, 64)])
+def test_routers_of_512_and_of_1024_threads(D, E):
+    """The last width that 512 threads read in one step, the first that they do not, and
+    one that takes 1024 threads two."""
+    t = make(9, D, 40, E, torch.float16, bias=True)
+    got = moe_ffn(**t, top_k=5, return_routing=True)
+    ref.check(got, ref.moe(**t, top_k=5))
+
+
 def test_one_expert_given_by_a_view():
     """E = 1: the expert pitch of a view plays no part."""
     t = make(3, 64, 40, 1, torch.bfloat16)
