@@ -31,8 +31,8 @@
 //     of phase 2 already on their way.
 //
 // Both launches (us, weights from HBM; the chosen experts' bytes at the measured copy
-// rate): 1 token, 2 of 8 experts of 4096 x 14336 122 (108); 8 tokens, 8 of 64 of 2048 x
-// 1024 99 (81); 64 tokens of the same 150 (123); 33 tokens, 4 of 16 of 1032 x 2824 75 (43).
+// rate): 1 token, 2 of 8 experts of 4096 x 14336 120 (108); 8 tokens, 8 of 64 of 2048 x
+// 1024 95 (81); 64 tokens of the same 151 (123); 33 tokens, 4 of 16 of 1032 x 2824 71 (43).
 //
 // Every wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once
@@ -251,7 +251,7 @@ struct MoeShape {
   static constexpr int BOX_BYTES = 64 * BK * 2;  // [64 k x 64 n]
   static constexpr int W_BYTES = 4 * BOX_BYTES;  // 256 columns
   // 128 KB of weights in flight an SM; more of them only wait for one another (8
-  // tokens, 64 experts: 99 us with 4 stages, 102 with 5, 104 with 6, 110 with 2).
+  // tokens, 64 experts: 3 us longer with 5 stages, 5 with 6, 11 with 2).
   static constexpr int MAX_STAGES = 4;
   static constexpr int THREADS = 192;
   // Behind the ring (W tiles, then token tiles):
@@ -362,8 +362,8 @@ __device__ __forceinline__ MoePhase moe_phase(const MoeParams& p, int chosen, bo
 }
 
 // Counts a CTA in: what it wrote before, and what threads wrote that it met at a barrier
-// since, is seen by whoever sees the count.  (One release for the CTA: a fence by each
-// of 128 threads takes some 2 us.)
+// since, is seen by whoever sees the count.  (One release for the CTA: with a fence
+// by each of 128 threads a call took 1.2 to 1.8 us longer.)
 __device__ __forceinline__ void moe_arrive(int* ctr) {
   asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(ctr) : "memory");
 }
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
     if (lane == 0) {
       // One thread feeds the SM, so it steps through runs and counts stages: with
       // the divisions of MoePhase::item per unit it was what bound the kernel (8
-      // tokens, 64 experts: 122 us, 145 with two more divisions).
+      // tokens, 64 experts: 23 us longer with two more divisions).
       struct Cursor {
         MoeRun r;
         int at, i;  // the run's position in the phase, the block within the run
