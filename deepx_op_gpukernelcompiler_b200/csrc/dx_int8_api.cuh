@@ -167,6 +167,9 @@ struct Int8Plan {
 //   evened out.  M = 64, N = 4096: 10.0 with 32 a tile against 11.6 with 64;
 //   M = 512: 17.2 with 64, 19.3 with 128; M = 1024: 24.9 with 128 against 33.5
 //   with 64, which make two waves.
+//   With several token tiles, clusters of 4 or more that leave an eighth of the wave
+//   free, or none: M = 80, K = N = 4096 11.6 with none, 15.1 with 3 CTAs; N = 3000,
+//   M = 96 14.8 with 4 CTAs in 97% of the wave, M = 128 11.5 with none.
 //   cluster: as many CTAs as fill a wave, up to 6, with some six K blocks each where
 //   there are that many; none where the tiles alone keep two thirds of the SMs busy.
 //   M = 1, weights from HBM: K = N = 4096 6.6-6.9 us for C = 4 to 8, 7.0-7.5 for 3
@@ -189,9 +192,9 @@ Int8Plan int8_tile_plan(const Int8Problem& p, int sms) {
   int64_t tiles = n_tiles * m_tiles;
   const int64_t k_blocks = (p.K + 127) / 128;
   const int64_t most = std::min<int64_t>(
-      std::min<int64_t>(6, 2 * sms / tiles),
+      std::min<int64_t>(6, (m_tiles > 1 ? 7 * sms / 4 : 2 * sms) / tiles),
       std::min<int64_t>(std::max<int64_t>(4, k_blocks / 6), k_blocks / 2));
-  if (3 * tiles < 2 * sms && most >= (m_tiles > 1 ? 3 : 2)) pl.cluster = static_cast<int>(most);
+  if (3 * tiles < 2 * sms && most >= (m_tiles > 1 ? 4 : 2)) pl.cluster = static_cast<int>(most);
   if (pl.cluster == 1 && tiles > sms && tiles <= 2 * sms) {
     // One or two CTAs an SM: the channels per tile that leave the busiest SM least.
     int64_t best = 2 * pl.nr;
@@ -369,12 +372,14 @@ void int8_pair_tiles(const Int8Problem& p, int workers, Int8Plan* pl) {
   }
 }
 
-// Pairs from 65 tokens on (us): M = 128, K = N = 4096: 11.5 against 12.3 for the
-// tile kernel; M = 256: 11.2 against 13.8; M = 64: 10.9 against 10.0, and with
-// N = 14336 17.9 against 14.2.
+// Pairs from 129 tokens on, gated from 65 (us, W from HBM, tile kernel against pairs).
+// M = 128: K = N = 4096 11.8 and 13.2; K x N = 14336 x 4096 29.4 and 32.8; 8192 x 28672
+// 49.3 and 53.8; 4096 x 14336 19.6 and 18.3.  M = 96: 4096 x 14336 17.4 and 18.3.
+// M = 256, K = N = 4096, W in L2: 13.8 and 11.2.  Gated, M = 64: 4096 x 14336 28.8 and
+// 32.4; 2056 x 5464 16.6 and 15.1; M = 128: 37.2 and 31.3, 22.0 and 15.2.
 Int8Plan int8_plan(const Int8Problem& p, int dev, int sms) {
   Int8Plan pl = int8_tile_plan(p, sms);
-  if (p.kernel == DX_KERNEL_DECODE || (p.kernel == DX_KERNEL_AUTO && p.M <= 64)) return pl;
+  if (p.kernel == DX_KERNEL_DECODE || (p.kernel == DX_KERNEL_AUTO && p.M <= (p.gated ? 64 : 128))) return pl;
   const int slots = std::min(pair_slots<256, __nv_bfloat16>(dev, sms), sms / 2);
   if (slots < 1) return pl;
   pl.pair = true;
