@@ -11,12 +11,12 @@
 //
 //   int8_pair_kernel  CTA pairs, 256 x bn tiles, persistent: the integer form
 //     of umma2_fused_linear_kernel (same roles, barriers and raster).  Serves
-//     more than 64 tokens.
+//     more than 128 tokens (gated: 64).
 //   int8_tile_kernel  one 128 (channels) x mn (tokens) tile per CTA with the
 //     operands swapped — D^T[n, m] — so that a few tokens cost a narrow MMA
 //     while W streams past once; K split over a cluster of C CTAs that add
 //     their integer partial sums through distributed shared memory.  Integer
-//     sums do not depend on their order.  Serves up to 64 tokens.
+//     sums do not depend on their order.  Serves up to 128 tokens (gated: 64).
 //
 // Every mbarrier wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once
