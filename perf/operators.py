@@ -102,11 +102,10 @@ def prepare(case, seed):
         return (torch.randn(shape, generator=gen, device=dev) * std).to(dt)
 
     def weight(n, k):
-        # 8-bit weights as a program keeps them: [channels, K] with rows padded to 16 bytes, and
-        # a scale for each channel.
-        q = torch.empty((n, -(-k // 16) * 16), dtype=torch.int8, device=dev)[:, :k]
-        q.copy_(torch.randn((n, k), generator=gen, device=dev).mul_(32).round_().clamp_(-127, 127))
-        return q, (torch.rand((n,), generator=gen, device=dev) + 0.5) / (32 * math.sqrt(k))
+        # 8-bit weights as a checkpoint holds them: [channels, K] and a scale for each channel.
+        q = torch.randn((n, k), generator=gen, device=dev).mul_(32).round_().clamp_(-127, 127)
+        s = (torch.rand((n,), generator=gen, device=dev) + 0.5) / (32 * math.sqrt(k))
+        return q.to(torch.int8), s
 
     if case["op"] == "moe":
         T, D, H, E = case["T"], case["D"], case["H"], case["E"]
