@@ -81,6 +81,7 @@ SIGNATURES = {
     "dx_fused_gated_linear_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, ctypes.c_int,
                                                                ctypes.c_int]),
     "dx_quantize_rows": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int, _vp]),
+    "dx_pack_int8_rows": (ctypes.c_int, [_vp, _vp] + [_i64] * 4 + [_vp]),
     "dx_int8_linear": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp]
                        + [_i64] * 7 + [ctypes.c_int] * 3 + [_vp, ctypes.c_size_t, _vp]),
     "dx_int8_gated_linear": (ctypes.c_int, [_vp, ctypes.c_int] + [_vp] * 8 + [_i64] * 7

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "dx_int8.cuh"
+#include "dx_pack.cuh"
 #include "dx_quant.cuh"
 
 namespace {
@@ -450,6 +451,41 @@ int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K,
   int rc = device_sms(dev, &sms);
   if (rc) return rc;
   return run_quantize(X, Q, scale, M, K, ldx, ldq, dtype, sms, static_cast<cudaStream_t>(stream));
+}
+
+int dx_pack_int8_rows(const void* src, void* dst, int64_t rows, int64_t K, int64_t ld_src,
+                      int64_t ld_dst, void* stream) {
+  t_last_error.clear();
+  if (rows < 0 || K < 0)
+    return fail(DX_ERR_INVALID_ARGUMENT, "negative shape rows=%lld K=%lld", (long long)rows,
+                (long long)K);
+  if (rows > 0x7fffffffLL || K > 0x3fffffffLL)
+    return fail(DX_ERR_UNSUPPORTED, "rows above 2^31-1 or K above 2^30-1");
+  if (rows == 0 || K == 0) return DX_OK;
+  if (src == nullptr || dst == nullptr)
+    return fail(DX_ERR_INVALID_ARGUMENT, "src or dst is NULL");
+  if (ld_src < K || ld_dst < round_up(K, 16))
+    return fail(DX_ERR_INVALID_ARGUMENT, "ld_src=%lld or ld_dst=%lld too small for K=%lld",
+                (long long)ld_src, (long long)ld_dst, (long long)K);
+  if (!aligned16(dst) || ld_dst % 16 != 0)
+    return fail(DX_ERR_INVALID_ARGUMENT, "dst needs a 16-byte-aligned pointer and pitch");
+  dx::PackParams p{};
+  p.src = static_cast<const uint8_t*>(src);
+  p.dst = static_cast<uint8_t*>(dst);
+  p.rows = static_cast<int>(rows);
+  p.K = static_cast<int>(K);
+  p.chunks = static_cast<int>((K + 15) / 16);
+  p.rows_per_cta = std::max(1, dx::kPackThreads * dx::kPackBatch / p.chunks);
+  p.ld_src = ld_src;
+  p.ld_dst = ld_dst;
+  const int grid = static_cast<int>((rows + p.rows_per_cta - 1) / p.rows_per_cta);
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = launch_config(grid, dx::kPackThreads, 0,
+                                         static_cast<cudaStream_t>(stream), 1, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, dx::pack_rows_kernel, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "launch pack_rows_kernel");
+  return DX_OK;
 }
 
 size_t dx_int8_workspace_size(int64_t M, int64_t K) {

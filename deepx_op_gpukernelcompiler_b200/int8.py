@@ -16,8 +16,11 @@ output channel and are held as [N, K]: the transpose of the 16-bit layers' W.
 
 X of a product is an Int8Rows pair or a floating-point matrix, which the call
 quantises first (one launch of its own, whose end overlaps the product's first
-loads of W).  The sums are exact: 32-bit integers, rounded to fp32 once and to
-the output type once.  Inference only: no gradients.
+loads of W).  A weight may be any pair of int8 rows and scales: rows that do not
+start on 16 bytes are copied to rows that do by the call itself, in every call (one
+launch, and N x K bytes of workspace); int8_rows does that once.  The sums are exact:
+32-bit integers, rounded to fp32 once and to the output type once.  Inference only:
+no gradients.
 """
 from __future__ import annotations
 
@@ -100,8 +103,9 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 
-def _pair(name: str, rows, K: int | None, n: int | None) -> tuple:
-    """Checks an (int8 rows, scales) pair -> (q, scale, rows, K, pitch)."""
+def _pair(name: str, rows, K: int | None, n: int | None, any_rows: bool = False) -> tuple:
+    """Checks an (int8 rows, scales) pair -> (q, scale, rows, K, pitch).  With
+    `any_rows` its rows may start anywhere (_packed lays them out)."""
     if not isinstance(rows, tuple) or len(rows) != 2:
         raise TypeError(f"{name} must be a pair (int8 rows, float32 scales), see quantize_rows")
     q, scale = rows
@@ -121,10 +125,24 @@ def _pair(name: str, rows, K: int | None, n: int | None) -> tuple:
         raise ValueError(f"{name}'s scales are on {scale.device}, its rows on {q.device}")
     if rows_ <= 1:
         ld = -(-cols // 16) * 16
-    if ld % 16 or q.data_ptr() % 16:
+    if not any_rows and (ld % 16 or q.data_ptr() % 16):
         raise ValueError(f"{name}'s rows must start on 16 bytes (pitch {ld}): int8_rows(q, scale) "
                          f"lays them out")
     return q, scale, rows_, cols, ld
+
+
+def _packed(lib, q: torch.Tensor, rows: int, K: int, ld: int, stream) -> tuple:
+    """Rows of a weight that start on 16 bytes -> (rows, address, pitch): its own, or
+    a copy of this call's (to be kept until the product is launched)."""
+    ptr = q.data_ptr()
+    if not (ld % 16 or ptr % 16):
+        return q, ptr, ld
+    pitch = -(-K // 16) * 16
+    space = q.new_empty(rows * pitch)
+    rc = lib.dx_pack_int8_rows(ptr, space.data_ptr(), rows, K, max(ld, K), pitch, stream)
+    if rc:
+        nat.check("dx_pack_int8_rows", rc)
+    return space, space.data_ptr(), pitch
 
 
 def _float_or_pair(X, dtype):
@@ -215,12 +233,13 @@ def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
     """Y = act(X Wq^T + bias) + residual on 8-bit operands (dx_int8_linear).
 
     X: a floating-point matrix [M, K] (quantised here, a scale per token) or an
-    Int8Rows pair.  W: an Int8Rows pair [N, K] (quantize_weight).  Y has X's type,
-    or `dtype` (bfloat16 by default where X is a pair); bias, residual and out
-    have Y's."""
+    Int8Rows pair.  W: a pair of int8 rows [N, K] and their scales (quantize_weight;
+    rows that do not start on 16 bytes cost a copy in every call, see int8_rows).  Y
+    has X's type, or `dtype` (bfloat16 by default where X is a pair); bias, residual
+    and out have Y's."""
     act, kcode = activation_code(activation), _kernel(kernel)
     x, x_code, x_scale, M, K, ldx, dtype = _float_or_pair(X, dtype)
-    wq, ws, N, _, ldw = _pair("W", W, K, None)
+    wq, ws, N, _, ldw = _pair("W", W, K, None, True)
     out, ldy = _output("int8_linear", out, x, M, N, dtype)
     index = x.get_device()
     _same_device(x, index, ("W", wq))
@@ -243,9 +262,10 @@ def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
             ws_bytes = lib.dx_int8_workspace_size(M, K)
             space = x.new_empty(ws_bytes, dtype=torch.uint8)
             ws_ptr = space.data_ptr()
+        w_rows, w_ptr, w_ld = _packed(lib, wq, N, K, ldw, stream)
         return lib.dx_int8_linear(
-            x.data_ptr(), x_code, sx_ptr, wq.data_ptr(), ws.data_ptr(), b_ptr, r_ptr,
-            out.data_ptr(), M, N, K, ldx, ldw, ldr, ldy, DTYPE_CODES[dtype], act, kcode, ws_ptr,
+            x.data_ptr(), x_code, sx_ptr, w_ptr, ws.data_ptr(), b_ptr, r_ptr,
+            out.data_ptr(), M, N, K, ldx, w_ld, ldr, ldy, DTYPE_CODES[dtype], act, kcode, ws_ptr,
             ws_bytes, stream)
 
     rc = _on_device(index, call)
@@ -262,8 +282,8 @@ def int8_gated_linear(X, Wg, Wu, bias_g: torch.Tensor | None = None,
     once for both weights (dx_int8_gated_linear).  Arguments as int8_linear."""
     act, kcode = activation_code(activation), _kernel(kernel)
     x, x_code, x_scale, M, K, ldx, dtype = _float_or_pair(X, dtype)
-    gq, gs, N, _, ldg = _pair("Wg", Wg, K, None)
-    uq, us, _, _, ldu = _pair("Wu", Wu, K, N)
+    gq, gs, N, _, ldg = _pair("Wg", Wg, K, None, True)
+    uq, us, _, _, ldu = _pair("Wu", Wu, K, N, True)
     out, ldy = _output("int8_gated_linear", out, x, M, N, dtype)
     index = x.get_device()
     _same_device(x, index, ("Wg", gq), ("Wu", uq))
@@ -279,9 +299,11 @@ def int8_gated_linear(X, Wg, Wu, bias_g: torch.Tensor | None = None,
             ws_bytes = lib.dx_int8_workspace_size(M, K)
             space = x.new_empty(ws_bytes, dtype=torch.uint8)
             ws_ptr = space.data_ptr()
+        g_rows, g_ptr, g_ld = _packed(lib, gq, N, K, ldg, stream)
+        u_rows, u_ptr, u_ld = _packed(lib, uq, N, K, ldu, stream)
         return lib.dx_int8_gated_linear(
-            x.data_ptr(), x_code, sx_ptr, gq.data_ptr(), gs.data_ptr(), uq.data_ptr(),
-            us.data_ptr(), bg_ptr, bu_ptr, out.data_ptr(), M, N, K, ldx, ldg, ldu, ldy,
+            x.data_ptr(), x_code, sx_ptr, g_ptr, gs.data_ptr(), u_ptr,
+            us.data_ptr(), bg_ptr, bu_ptr, out.data_ptr(), M, N, K, ldx, g_ld, u_ld, ldy,
             DTYPE_CODES[dtype], act, kcode, ws_ptr, ws_bytes, stream)
 
     rc = _on_device(index, call)

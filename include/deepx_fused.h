@@ -296,6 +296,14 @@ size_t dx_fused_gated_linear_workspace_size(int64_t M, int64_t N, int64_t K,
 int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K, int64_t ldx,
                      int64_t ldq, int dtype, void* stream);
 
+/* Copies `rows` rows of K bytes, at any pitch and alignment, to rows that start on
+ * 16 bytes (dst 16-byte-aligned, ld_dst a multiple of 16, at least K rounded up to
+ * one): the layout that the products below take, for 8-bit weights or activations
+ * that lie otherwise.  Whole 16-byte pieces of dst are written, with any values
+ * behind K.  Bytes between src's first and last row may be read. */
+int dx_pack_int8_rows(const void* src, void* dst, int64_t rows, int64_t K, int64_t ld_src,
+                      int64_t ld_dst, void* stream);
+
 /*
  * Y = act(x_scale[m] w_scale[n] sum_k Xq[m,k] Wq[n,k] + bias[n]) + R[m,n].
  * X is 8-bit with its scales (x_dtype = DX_DTYPE_I8; 16-byte-aligned, ldx a
