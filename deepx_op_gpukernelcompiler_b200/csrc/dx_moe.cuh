@@ -41,6 +41,7 @@
 #include <type_traits>
 
 #include "dx_epilogue.cuh"
+#include "dx_moe_plan.cuh"
 #include "dx_ptx.cuh"
 
 namespace dx {
@@ -48,7 +49,6 @@ namespace dx {
 constexpr int kMoeMaxT = 64;
 constexpr int kMoeMaxE = 256;
 constexpr int kMoeMaxTop = 32;
-constexpr int kMoeWholeBlocks = 10;
 
 // ---------------------------------------------------------------- router
 constexpr int kRouterTokens = 8;  // tokens of a cluster = its CTAs
@@ -242,7 +242,7 @@ struct MoeParams {
   void* Y;
   long long ldy;
   void *h_hi, *h_lo;  // [chosen experts][T][H]
-  float* partials;    // [CTA][first / later tile][2][T][128]
+  float* partials;    // [CTA][kMoeSlots][2][T][128]
   int* counters;      // [2 phases][CTA] tile arrivals, then the phase barrier; zero before
 };
 
@@ -276,90 +276,6 @@ struct MoeShape {
     return n < MAX_STAGES ? n : MAX_STAGES;
   }
 };
-
-// A run of K blocks that one accumulator collects: of one tile (phase 1), or of
-// one tile and one expert (phase 2).
-struct MoeRun {
-  int tile, a, kb0, len;  // a: index into the chosen experts
-};
-
-// One phase's work of one CTA.  The `tiles - whole` tiles that do not make a full
-// wave of the grid are dealt out first, as units of one K block, evenly and
-// contiguously (a CTA gets parts of at most a few tiles); then come full waves of
-// whole tiles, whose epilogues need nobody else.  So the exchange of partial sums
-// runs beside the streaming of whole tiles, where a phase has any (phase 1 of
-// 8 tokens, 64 experts of 2048 x 1024: 336 tiles on 148 CTAs).
-struct MoePhase {
-  int tiles, whole, per_tile;  // tiles [0, whole) are whole; units of a tile
-  int each, more;              // split units of a CTA; the first `more` CTAs have one more
-  int nt, kb;                  // phase 1: tiles of an expert; K blocks of an expert's product
-  int u0, u1;                  // this CTA's units
-  bool second;
-
-  __device__ __forceinline__ int begin(int g) const { return g * each + min(g, more); }
-  __device__ __forceinline__ int cta_of(int u) const {
-    const int front = more * (each + 1);
-    return u < front ? u / (each + 1) : more + (u - front) / each;
-  }
-  // The work item at position i of this CTA's list (its units, then the units of
-  // its whole tiles): tile, expert index and K block.
-  __device__ __forceinline__ int count() const {
-    const int mine = whole > static_cast<int>(blockIdx.x)
-                         ? (whole - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1
-                         : 0;
-    return u1 - u0 + mine * per_tile;
-  }
-  __device__ __forceinline__ void item(int i, int& tile, int& a, int& kb_) const {
-    int r;
-    if (i < u1 - u0) {
-      const int u = u0 + i;
-      tile = u / per_tile;
-      r = u - tile * per_tile;
-      tile += whole;
-    } else {
-      i -= u1 - u0;
-      const int w = i / per_tile;
-      r = i - w * per_tile;
-      tile = static_cast<int>(blockIdx.x) + w * static_cast<int>(gridDim.x);
-    }
-    if (second) {
-      a = r / kb;
-      kb_ = r - a * kb;
-    } else {
-      a = tile / nt;
-      kb_ = r;
-    }
-  }
-  __device__ __forceinline__ bool run(int i, MoeRun& r) const {
-    if (i >= count()) return false;
-    item(i, r.tile, r.a, r.kb0);
-    r.len = kb - r.kb0;
-    if (i < u1 - u0) r.len = min(r.len, u1 - u0 - i);
-    return true;
-  }
-};
-
-__device__ __forceinline__ MoePhase moe_phase(const MoeParams& p, int chosen, bool second) {
-  MoePhase f;
-  const int grid = static_cast<int>(gridDim.x), g = static_cast<int>(blockIdx.x);
-  f.second = second;
-  f.kb = second ? p.kb_h : p.kb_d;
-  f.nt = p.nt_h;
-  f.per_tile = second ? chosen * p.kb_h : p.kb_d;
-  f.tiles = second ? p.nt_d : chosen * p.nt_h;
-  f.whole = f.tiles / grid * grid;
-  // Fewer tiles than CTAs, and short ones: joining partial sums costs more than the K
-  // blocks it saves the CTAs that have a tile (20 tokens, 2 of 60 experts of 1024 x 512:
-  // 32.4 us whole, 35.1 split; 1 token, 1 of 8 of 2048 x 4096: 42.6 and 27.1).
-  if (!second && f.whole == 0 && f.per_tile - f.tiles * f.per_tile / grid <= kMoeWholeBlocks)
-    f.whole = f.tiles;
-  const int units = (f.tiles - f.whole) * f.per_tile;
-  f.each = units / grid;
-  f.more = units - f.each * grid;
-  f.u0 = f.begin(g);
-  f.u1 = f.begin(g + 1);
-  return f;
-}
 
 // Counts a CTA in: what it wrote before, and what threads wrote that it met at a barrier
 // since, is seen by whoever sees the count.  (One release for the CTA: with a fence
@@ -667,9 +583,9 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
     auto chosen_by = [&](int e) {  // the tokens of expert e
       return s_mask[2 * e] | (static_cast<unsigned long long>(s_mask[2 * e + 1]) << 32);
     };
-    // Partial sums of a CTA's first tile (slot 0) or of its last (slot 1): [2][T][128].
+    // A slot of a CTA's partial sums (MoePhase::slot): [2][T][128].
     const long long slot_floats = static_cast<long long>(2 * p.T) * 128;
-    auto part = [&](int cta, int slot) { return p.partials + (cta * 2 + slot) * slot_floats; };
+    auto part = [&](int cta, int slot) { return p.partials + (cta * kMoeSlots + slot) * slot_floats; };
     // The tile whose partial sums this CTA has just written: `peers` CTAs from
     // `first` on have a share of it, `sum` points at the first one's, and this CTA
     // finishes every shares'th row from `share` on (-1: none).  Counts the CTA in;
@@ -687,8 +603,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         peers = last - first + 1;
         shares = last - first + (f.begin(last + 1) == ue ? 1 : 0);
         share = f.u1 <= ue ? g - first : -1;
-        // (a CTA that starts inside the tile has it as its first tile)
-        if (first != g) slot = f.begin(first) / f.per_tile == tile - f.whole ? 0 : 1;
+        if (first != g) slot = f.slot_of(first, tile);
       }
       sum = part(first, slot);
       named_bar_sync(1, 128);
@@ -718,7 +633,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
           for (int j = 0; j < kRows; ++j)
             v[k][j] = i + k < peers - 1
                           ? __ldcg(reinterpret_cast<const float4*>(
-                                next + 2 * slot_floats * (i + k) + j * apart * 128))
+                                next + kMoeSlots * slot_floats * (i + k) + j * apart * 128))
                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
@@ -741,7 +656,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         const int col0 = (r.tile - r.a * f.nt) * 128;
         const unsigned long long mask = chosen_by(e);
         const bool whole = r.len == f.per_tile;
-        const int slot = f.u0 / f.per_tile + f.whole == r.tile ? 0 : 1;
+        const int slot = f.slot(r.tile, whole);
         const bool live = col0 + n < p.H;
         float vg = 0.0f, vu = 0.0f;
         if (whole && live) {
@@ -901,7 +816,7 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
         if (f.run(u + r.len, after) && after.tile == r.tile) continue;
         const int us = (r.tile - f.whole) * f.per_tile;
         const bool whole = r.tile < f.whole || (f.u0 <= us && f.u1 >= us + f.per_tile);
-        const int slot = r.tile >= f.whole && f.u0 / f.per_tile + f.whole == r.tile ? 0 : 1;
+        const int slot = f.slot(r.tile, whole);
         float* const to = part(g, slot) + n;
         float* const to1 = to + p.T * 128;
 #pragma unroll

@@ -26,7 +26,8 @@ MoeLayout moe_layout(int64_t T, int64_t H, int64_t E, int64_t top, int ctas) {
     return at;
   };
   l.h = place(static_cast<size_t>(l.chosen * T * H) * 2 * 2);
-  l.partials = place(static_cast<size_t>(ctas) * 2 * 2 * static_cast<size_t>(T) * 128 * sizeof(float));
+  l.partials = place(static_cast<size_t>(ctas) * dx::kMoeSlots * 2 * static_cast<size_t>(T) * 128 *
+                     sizeof(float));
   l.num_counters = 2 * ctas + 1;
   l.counters = place(static_cast<size_t>(l.num_counters) * sizeof(int));
   return l;
