@@ -98,11 +98,6 @@ def int8_rows(q: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
     return Int8Rows(q, scale.contiguous())
 
 
-# The current stream's handle without building a Stream object (2 us a call).
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
-
-
 def _pair(name: str, rows, K: int | None, n: int | None, any_rows: bool = False) -> tuple:
     """Checks an (int8 rows, scales) pair -> (q, scale, rows, K, pitch).  With
     `any_rows` its rows may start anywhere (_packed lays them out)."""
@@ -221,10 +216,12 @@ def _vector(name: str, b: torch.Tensor | None, N: int, x: torch.Tensor, dtype: t
 
 def _on_device(index: int, call):
     """call(stream) with device `index` current; `stream` is its current stream's handle."""
-    if index == _current_device():
-        return call(_raw_stream(index))
+    # torch._C's own functions: building a Stream object takes 2 us a call.  Looked up
+    # here, since a torch without CUDA does not have them.
+    if index == torch._C._cuda_getDevice():
+        return call(torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
-        return call(_raw_stream(index))
+        return call(torch._C._cuda_getCurrentRawStream(index))
 
 
 def int8_linear(X, W, bias: torch.Tensor | None = None, activation=None,
