@@ -9,7 +9,7 @@
 // Two launches:
 //
 //   moe_router_kernel  clusters of 8 CTAs, 8 tokens each: the CTAs split D, add
-//     their fp32 partial logits through distributed shared memory, and CTA i
+//     their 64-bit partial logits through distributed shared memory, and CTA i
 //     picks token i's experts.
 //   moe_experts_kernel  one CTA per SM, all resident (cooperative launch).
 //     Phase 1 computes h = act(gate) * up of every chosen expert, phase 2 the
@@ -37,7 +37,6 @@
 // Every wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once
 
-#include <algorithm>
 #include <type_traits>
 
 #include "dx_epilogue.cuh"
@@ -52,17 +51,9 @@ constexpr int kMoeMaxTop = 32;
 
 // ---------------------------------------------------------------- router
 constexpr int kRouterTokens = 8;  // tokens of a cluster = its CTAs
-constexpr int kRouterRows = 512;  // rows of Wr per step, at most
-constexpr int kRouterBatch = 16;  // rows of Wr a thread, per step
-// Threads of a CTA: 1024, or 512 where those read their share of Wr in one step as well
-// (a call 1.0 to 1.4 us shorter, of 17 to 48: half as many sums to add; 0.3 to 1.1 us
-// longer where it takes them a second step).
-constexpr int router_threads(int D, int E) {
-  return (D + kRouterTokens - 1) / kRouterTokens <=
-                 std::min(kRouterRows, kRouterBatch * (512 / ((E + 31) / 32 * 32)))
-             ? 512
-             : 1024;
-}
+constexpr int kRouterThreads = 512;
+constexpr int kRouterBlock = 32;  // rows of Wr that a warp's loads cover at once
+constexpr int kRouterBatch = 4;   // such blocks on their way to a warp, a sum each
 
 struct MoeRouterParams {
   const void* X;
@@ -76,107 +67,94 @@ struct MoeRouterParams {
   int num_counters;
 };
 
-// Unsigned key in the order of the floats (a NaN sorts by its sign and bits).
-__device__ __forceinline__ uint32_t moe_key(float f) {
-  const uint32_t u = __float_as_uint(f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// Unsigned key in the order of the doubles (a NaN sorts by its sign and bits).
+__device__ __forceinline__ unsigned long long moe_key(double f) {
+  const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(f));
+  return (u >> 63) != 0 ? ~u : (u | (1ull << 63));
 }
 
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) moe_router_kernel(const MoeRouterParams p) {
+// The logits are sums in 64 bits: which experts are chosen is decided next to a
+// border, where fp32 sums may order two of them otherwise.  8 tokens x 8 experts x 4
+// rows are one 64-bit matrix instruction (tcgen05 has none of that type), to which a
+// lane gives one value of X and one of Wr, straight from memory.  Sums by multiply-adds,
+// a thread an expert, are bound by the tokens' values coming out of shared memory: the
+// layer for 8 tokens, 64 experts of 4096 x 256 took 62.6 us with fp32 ones, 71.7 with
+// 64-bit ones, 61.2 with this; 8 tokens, 64 of 2048 x 1024 92.3, 98.9 and 92.2.
+template <typename T>
+__global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeRouterParams p) {
   using Tr = ElemTraits<T>;
-  __shared__ __align__(16) float s_x[THREADS][kRouterTokens];  // [row][token]
-  static_assert(kRouterRows <= THREADS, "a step's rows");
-  float* const s_part = &s_x[0][0];  // [row group][token][expert], once s_x is done with
-  __shared__ float s_sum[kRouterTokens][kMoeMaxE];
-  __shared__ float s_logit[kMoeMaxE];
+  constexpr int kWarps = kRouterThreads / 32;
+  __shared__ double s_part[kMoeMaxE / 8][kRouterTokens][8];  // [row group, 8 experts][token][expert]
+  static_assert(kMoeMaxE / 8 >= kWarps, "a part for each warp");
+  __shared__ double s_sum[kRouterTokens][kMoeMaxE];
+  __shared__ double s_logit[kMoeMaxE];
   const int tid = static_cast<int>(threadIdx.x);
+  const int warp = tid >> 5, lane = tid & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int t0 = static_cast<int>(blockIdx.x) / kRouterTokens * kRouterTokens;
   const int tokens = min(kRouterTokens, p.T - t0);
   grid_dependency_wait();
   grid_launch_dependents();
   if (blockIdx.x == 0)
-    for (int i = tid; i < p.num_counters; i += THREADS) p.counters[i] = 0;
+    for (int i = tid; i < p.num_counters; i += kRouterThreads) p.counters[i] = 0;
 
-  // Threads as row groups x experts; each sums its rows for all tokens.  Wr's rows
-  // are asked for before the tokens' values are needed: one trip to memory a step.
-  const int ep = (p.E + 31) / 32 * 32;
-  const int groups = THREADS / ep;
-  const int e = tid % ep, kg = tid / ep;
-  const bool live = kg < groups && e < p.E;
-  const int slice = (p.D + kRouterTokens - 1) / kRouterTokens;
+  // This CTA's rows of Wr, a multiple of 8; warps as row groups x tiles of 8 experts.
+  const int slice = ((p.D + kRouterTokens - 1) / kRouterTokens + 7) / 8 * 8;
   const int k_begin = rank * slice, k_end = min(p.D, k_begin + slice);
-  const T* const X = static_cast<const T*>(p.X);
-  const T* const Wr = static_cast<const T*>(p.Wr);
-  constexpr int kBatch = kRouterBatch;
-  constexpr int kPerThread = kRouterRows * kRouterTokens / THREADS;  // token values
-  const int step = min(kRouterRows, kBatch * groups);  // rows of Wr per step
-  float acc[kRouterTokens];
+  const int tiles = (p.E + 7) / 8;
+  const int across = min(tiles, kWarps), groups = kWarps / across;
+  const int group = warp / across;
+  const int m = lane >> 2, j = lane & 3;  // the lane's token and expert of 8; its rows, 8 j on
+  if (group < groups) {
+    const T* const x_row = static_cast<const T*>(p.X) + static_cast<long long>(t0 + m) * p.ldx;
+    for (int tile = warp % across; tile < tiles; tile += across) {
+      const int e = tile * 8 + m;
+      const T* const w_col = static_cast<const T*>(p.Wr) + e;
+      double c[kRouterBatch][2] = {};  // (sums that do not wait for one another)
+      for (int k0 = k_begin + group * kRouterBlock; k0 < k_end;
+           k0 += groups * kRouterBlock * kRouterBatch) {
+        T w[kRouterBatch][8];
+        __align__(16) T x[kRouterBatch][8];
 #pragma unroll
-  for (int t = 0; t < kRouterTokens; ++t) acc[t] = 0.0f;
-  for (int k0 = k_begin; k0 < k_end; k0 += step) {
-    const int rows = min(step, k_end - k0);
-    T w[kBatch], x[kPerThread];
+        for (int i = 0; i < kRouterBatch; ++i) {
+          const int k = k0 + i * groups * kRouterBlock + 8 * j;
+          const bool in = k < k_end;  // (all eight rows or none)
+          *reinterpret_cast<uint4*>(x[i]) = in && m < tokens
+                                                ? *reinterpret_cast<const uint4*>(x_row + k)
+                                                : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      const int at = i * THREADS + tid, t = at / kRouterRows, k = at % kRouterRows;
-      x[i] = t < tokens && k < rows ? X[(t0 + t) * p.ldx + k0 + k] : Tr::from_float(0.0f);
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int k = kg + i * groups;
-      w[i] = live && k < rows ? Wr[(k0 + k) * p.ldwr + e] : Tr::from_float(0.0f);
-    }
-    if (k0 != k_begin) __syncthreads();  // the previous step's values are no longer read
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      const int at = i * THREADS + tid;
-      s_x[at % kRouterRows][at / kRouterRows] = Tr::to_float(x[i]);
-    }
-    __syncthreads();
-    if (live) {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int k = kg + i * groups;
-        if (k < rows) {
-          const float f = Tr::to_float(w[i]);
-          const float4 a = *reinterpret_cast<const float4*>(&s_x[k][0]);
-          const float4 b = *reinterpret_cast<const float4*>(&s_x[k][4]);
-          acc[0] = fmaf(a.x, f, acc[0]);
-          acc[1] = fmaf(a.y, f, acc[1]);
-          acc[2] = fmaf(a.z, f, acc[2]);
-          acc[3] = fmaf(a.w, f, acc[3]);
-          acc[4] = fmaf(b.x, f, acc[4]);
-          acc[5] = fmaf(b.y, f, acc[5]);
-          acc[6] = fmaf(b.z, f, acc[6]);
-          acc[7] = fmaf(b.w, f, acc[7]);
+          for (int r = 0; r < 8; ++r)
+            w[i][r] = in && e < p.E ? w_col[(k + r) * p.ldwr] : Tr::from_float(0.0f);
         }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int i = 0; i < kRouterBatch; ++i)
+            mma_f64(c[i], static_cast<double>(Tr::to_float(x[i][r])),
+                    static_cast<double>(Tr::to_float(w[i][r])));
       }
+      double* const to = &s_part[group * tiles + tile][m][2 * j];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) to[h] = (c[0][h] + c[1][h]) + (c[2][h] + c[3][h]);
     }
   }
   __syncthreads();
-  if (kg < groups) {
-#pragma unroll
-    for (int t = 0; t < kRouterTokens; ++t) s_part[(kg * kRouterTokens + t) * ep + e] = acc[t];
-  }
-  __syncthreads();
-  for (int i = tid; i < kRouterTokens * ep; i += THREADS) {
-    const int t = i / ep, ee = i % ep;
-    float s = 0.0f;
-    for (int g = 0; g < groups; ++g) s += s_part[(g * kRouterTokens + t) * ep + ee];
-    s_sum[t][ee] = s;
+  for (int i = tid; i < tokens * p.E; i += kRouterThreads) {
+    const int t = i / p.E, e = i - t * p.E;
+    double s = 0.0;
+    for (int g = 0; g < groups; ++g) s += s_part[g * tiles + e / 8][t][e % 8];
+    s_sum[t][e] = s;
   }
   cluster_sync();
   const int token = t0 + rank;
   if (rank < tokens) {
-    for (int i = tid; i < p.E; i += THREADS) {
-      float s = 0.0f;
+    for (int i = tid; i < p.E; i += kRouterThreads) {
+      double s = 0.0;
 #pragma unroll
       for (int c = 0; c < kRouterTokens; ++c)
-        s += ld_shared_cluster_f32(
+        s += ld_shared_cluster_f64(
             mapa_shared(smem_u32(&s_sum[rank][i]), static_cast<uint32_t>(c)));
-      if (p.br != nullptr) s += Tr::to_float(static_cast<const T*>(p.br)[i]);
+      if (p.br != nullptr) s += static_cast<double>(Tr::to_float(static_cast<const T*>(p.br)[i]));
       s_logit[i] = s;
     }
   }
@@ -185,19 +163,23 @@ __global__ void __launch_bounds__(THREADS) moe_router_kernel(const MoeRouterPara
 
   // One warp: lane l holds experts l, l + 32, ...
   constexpr int kPer = kMoeMaxE / 32;
-  uint32_t key[kPer];  // 0: absent or taken (no float's key is 0 but a NaN's)
+  unsigned long long key[kPer];  // 0: absent or taken (no number's key is 0, a NaN's may be)
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int ee = i * 32 + tid;
-    key[i] = ee < p.E ? max(moe_key(s_logit[ee]), 1u) : 0u;
+    key[i] = ee < p.E ? max(moe_key(s_logit[ee]), 1ull) : 0ull;
   }
-  float top_logit = 0.0f, sum = 0.0f, mine = 0.0f;
+  double top_logit = 0.0;
+  float sum = 0.0f, mine = 0.0f;
   int my_id = 0;
   for (int j = 0; j < p.top; ++j) {
-    uint32_t best = 0;
+    unsigned long long best = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
-    best = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t high = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(best >> 32));
+    const uint32_t low = __reduce_max_sync(
+        0xffffffffu, static_cast<uint32_t>(best >> 32) == high ? static_cast<uint32_t>(best) : 0u);
+    best = (static_cast<unsigned long long>(high) << 32) | low;
     uint32_t at = kMoeMaxE;
 #pragma unroll
     for (int i = kPer - 1; i >= 0; --i)
@@ -206,9 +188,9 @@ __global__ void __launch_bounds__(THREADS) moe_router_kernel(const MoeRouterPara
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (i * 32 + tid == id) key[i] = 0;
-    const float l = s_logit[id];
+    const double l = s_logit[id];
     if (j == 0) top_logit = l;
-    const float x = expf(l - top_logit);
+    const float x = expf(static_cast<float>(l - top_logit));
     sum += x;
     if (tid == j) {
       mine = x;
@@ -217,7 +199,7 @@ __global__ void __launch_bounds__(THREADS) moe_router_kernel(const MoeRouterPara
   }
   if (!p.renormalize) {
     sum = 0.0f;
-    for (int ee = tid; ee < p.E; ee += 32) sum += expf(s_logit[ee] - top_logit);
+    for (int ee = tid; ee < p.E; ee += 32) sum += expf(static_cast<float>(s_logit[ee] - top_logit));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }

@@ -173,11 +173,9 @@ int launch_moe(const dx_moe_args& a, int dev, int ctas, const MoeLayout& l, cuda
   r.num_counters = l.num_counters;
   const int groups = (r.T + dx::kRouterTokens - 1) / dx::kRouterTokens;
   cudaLaunchAttribute attr[2];
-  const int threads = dx::router_threads(r.D, r.E);
-  cudaLaunchConfig_t cfg = launch_config(groups * dx::kRouterTokens, threads, 0, stream,
+  cudaLaunchConfig_t cfg = launch_config(groups * dx::kRouterTokens, dx::kRouterThreads, 0, stream,
                                          dx::kRouterTokens, attr);
-  cudaError_t e = threads == 512 ? cudaLaunchKernelEx(&cfg, dx::moe_router_kernel<T, 512>, r)
-                                 : cudaLaunchKernelEx(&cfg, dx::moe_router_kernel<T, 1024>, r);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, dx::moe_router_kernel<T>, r);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch moe_router_kernel");
   if (a.T <= 16) return launch_moe_experts<16, T>(a, dev, ctas, l, stream);

@@ -339,7 +339,7 @@ size_t dx_int8_workspace_size(int64_t M, int64_t K);
 /*
  * A mixture-of-experts layer for the tokens of a serving step (the reference
  * lists its chain, `moe_ffn`, as multi_kernel and never runs it):
- *   l = X Wr + br; each token's top_k experts by l, ties to the lowest number
+ *   l = X Wr + br (64-bit sums); each token's top_k experts by l, ties to the lowest number
  *   w_e = exp(l_e) / (sum over the chosen experts, or over all: renormalize = 0)
  *   Y = R + sum_e w_e ((act(X Wg[e] + bg[e]) * (X Wu[e] + bu[e])) Wo[e] + bo[e])
  * in two launches that read the weights of each chosen expert once.  fp16/bf16;
