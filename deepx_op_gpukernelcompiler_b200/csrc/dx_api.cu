@@ -156,7 +156,6 @@ int device_sms(int dev, int* sms) {
 PFN_cuStreamGetCtx_v12050 g_stream_ctx = nullptr;
 PFN_cuGreenCtxGetDevResource_v12040 g_green_res = nullptr;
 std::once_flag g_green_once;
-std::map<CUgreenCtx, int> g_green_sms;
 
 int stream_sms(cudaStream_t s, int dev, int* sms) {
   int rc = device_sms(dev, sms);
@@ -180,16 +179,10 @@ int stream_sms(cudaStream_t s, int dev, int* sms) {
   CUgreenCtx green = nullptr;
   if (g_stream_ctx(reinterpret_cast<CUstream>(s), &ctx, &green) != CUDA_SUCCESS || green == nullptr)
     return DX_OK;  // a regular context: the whole device
-  std::lock_guard<std::mutex> lk(g_mu);
-  auto it = g_green_sms.find(green);
-  if (it == g_green_sms.end()) {
-    CUdevResource r{};
-    int n = *sms;
-    if (g_green_res(green, &r, CU_DEV_RESOURCE_TYPE_SM) == CUDA_SUCCESS && r.sm.smCount > 0)
-      n = static_cast<int>(r.sm.smCount);
-    it = g_green_sms.emplace(green, n).first;
-  }
-  *sms = std::min(*sms, it->second);
+  // (asked for at every launch: a later context may have this one's handle)
+  CUdevResource r{};
+  if (g_green_res(green, &r, CU_DEV_RESOURCE_TYPE_SM) == CUDA_SUCCESS && r.sm.smCount > 0)
+    *sms = std::min(*sms, static_cast<int>(r.sm.smCount));
   return DX_OK;
 }
 
