@@ -21,6 +21,12 @@ int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 int elem_size(int dtype) { return dtype == DX_DTYPE_F32 ? 4 : 2; }
 
+// Whether every pointer is at a multiple of `size` bytes, as its elements have to be.
+template <typename... P>
+bool element_aligned(int size, P... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & static_cast<uintptr_t>(size - 1)) == 0;
+}
+
 bool float_dtype(int dtype) { return dtype >= DX_DTYPE_F32 && dtype <= DX_DTYPE_BF16; }
 
 // 8-bit matrix of `rows` rows of `k` bytes, a [box_rows x 128 byte] box.
@@ -146,6 +152,10 @@ int int8_validate(const Int8Problem& p) {
       (p.x_dtype == DX_DTYPE_I8 && (!aligned16(p.X) || p.ldx % 16 != 0)))
     return fail(DX_ERR_UNSUPPORTED,
                 "8-bit operands need 16-byte-aligned pointers and pitches that are multiples of 16");
+  if (!element_aligned(4, p.x_scale, p.w_scale, p.w2_scale) ||
+      !element_aligned(elem_size(p.dtype), p.bias, p.bias2, p.R, p.Y) ||
+      (p.x_dtype != DX_DTYPE_I8 && !element_aligned(elem_size(p.x_dtype), p.X)))
+    return fail(DX_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its elements");
   return DX_OK;
 }
 
@@ -444,6 +454,8 @@ int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K,
   if (ldx < K || ldq < K)
     return fail(DX_ERR_INVALID_ARGUMENT, "ldx=%lld or ldq=%lld below K=%lld", (long long)ldx,
                 (long long)ldq, (long long)K);
+  if (!element_aligned(elem_size(dtype), X) || !element_aligned(4, scale))
+    return fail(DX_ERR_INVALID_ARGUMENT, "X or scale is not aligned to its elements");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");

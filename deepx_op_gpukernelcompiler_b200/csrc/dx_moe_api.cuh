@@ -87,6 +87,9 @@ int moe_validate(const dx_moe_args* a) {
   if (a->E > 1 && (a->ldg_expert < a->ldg * a->D || a->ldu_expert < a->ldu * a->D ||
                    a->ldo_expert < a->ldo * a->H))
     return fail(DX_ERR_INVALID_ARGUMENT, "moe: an expert's pitch is below its matrix");
+  if (!element_aligned(2, a->Wr, a->br, a->bg, a->bu, a->bo, a->R, a->Y) ||
+      !element_aligned(4, a->ids, a->weights))
+    return fail(DX_ERR_INVALID_ARGUMENT, "moe: a pointer is not aligned to its elements");
   return DX_OK;
 }
 

@@ -290,8 +290,8 @@ size_t dx_fused_gated_linear_workspace_size(int64_t M, int64_t N, int64_t K,
  *
  * dx_quantize_rows: a = max(max_k |X[m,k]|, 2^-100), scale[m] = a / 127,
  * Q[m,k] = the integer nearest 127 X[m,k] / a, halves to even.  A row with an
- * infinity or NaN gets scale NaN and zeros.  Any pitch and alignment; bytes of
- * Q's rows behind K are left alone.
+ * infinity or NaN gets scale NaN and zeros.  Any pitch, and any alignment that
+ * the elements have; bytes of Q's rows behind K are left alone.
  */
 int dx_quantize_rows(const void* X, void* Q, float* scale, int64_t M, int64_t K, int64_t ldx,
                      int64_t ldq, int dtype, void* stream);
