@@ -21,9 +21,9 @@
 //     chosen expert — the MMA has columns to spare, and no gathering is needed —
 //     and the epilogue uses a token's column only where the token chose the
 //     expert, so nothing of an expert (an infinity, a NaN) reaches other tokens.
-//     h is kept as a sum of two 16-bit values (hi + lo, 16 or 22 bits), both
-//     multiplied by Wo: the second product is as exact as with fp32 h, at no
-//     cost beside the weights' stream.
+//     h is kept as two 16-bit values (MoeHidden), both multiplied by Wo: a relative
+//     error of 2^-17 (bf16) or 2^-22 (fp16), where one value has 2^-9 or 2^-12.  In
+//     fp16 it also has a step of 2^-36, and h has to stay below 65504.
 //     A tile that several CTAs share leaves fp32 partial sums; when all are
 //     there the CTAs that end in the tile finish a share of its rows each,
 //     adding the partials in CTA order (results do not depend on timing).
@@ -286,13 +286,22 @@ __device__ __forceinline__ bool moe_wait(const int* ctr, int target, volatile in
   }
 }
 
-// h as hi + lo of type T.
+// h as hi + lo / kScale of type T.  bf16's lo has the exponents it needs; fp16's is
+// kept 2^11 times as large, about as large as hi, so that it does not end among the
+// subnormals for every h below 2^-3, and has sums of its own in TMEM (X of scale 0.001
+// and Wo 4000 times as large as usual: outputs 3% of their norm off otherwise, 0.02% so).
+template <typename T>
+struct MoeHidden {
+  static constexpr bool kApart = !ElemTraits<T>::kIsBf16;
+  static constexpr float kScale = kApart ? 2048.0f : 1.0f;
+};
+
 template <typename T>
 __device__ __forceinline__ void moe_split(float h, T& hi, T& lo) {
   using Tr = ElemTraits<T>;
   hi = Tr::from_float(h);
   const float rest = h - Tr::to_float(hi);
-  lo = Tr::from_float(rest - rest == 0.0f ? rest : 0.0f);  // an infinite hi has no lo
+  lo = Tr::from_float(rest - rest == 0.0f ? rest * MoeHidden<T>::kScale : 0.0f);  // an infinite hi has no lo
 }
 
 template <typename T>
@@ -331,7 +340,9 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
   int* const s_chosen = reinterpret_cast<int*>(tail_ptr + S::OFF_MISC + 8);
   volatile int* const s_ok = reinterpret_cast<volatile int*>(tail_ptr + S::OFF_MISC + 12);
   auto bar = [bars](int i) { return bars + 8u * static_cast<uint32_t>(i); };
-  constexpr uint32_t kTmemCols = 4 * MN < 32 ? 32 : 4 * MN;  // two buffers x two halves
+  // Two buffers x two halves, then the same for the lo sums where they are apart.
+  constexpr bool kApart = MoeHidden<T>::kApart;
+  constexpr uint32_t kTmemCols = (kApart ? 8 : 4) * MN;
 
   const int tid = static_cast<int>(threadIdx.x);
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -530,7 +541,8 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
               if (ph != 0) {
 #pragma unroll
                 for (int k = 0; k < S::BK / 16; ++k)
-                  umma_f16(dh, wd + 128ull * k, lo + 2ull * k, idesc, 1u);
+                  umma_f16(kApart ? dh + 4 * MN : dh, wd + 128ull * k, lo + 2ull * k, idesc,
+                           (!kApart || i != 0 || k != 0) ? 1u : 0u);
               }
             }
             umma_commit(bar(S::BAR_EMPTY + s));
@@ -779,9 +791,17 @@ __global__ void __launch_bounds__(MoeShape::THREADS, 1)
               *reinterpret_cast<float4*>(w + j) = *reinterpret_cast<const float4*>(roww + mc + j);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint32_t v[16];
+              uint32_t v[16], l[kApart ? 16 : 1];
               tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(h * MN + mc), v);
+              if constexpr (kApart)
+                tmem_ld_32x32b_x16(acc + static_cast<uint32_t>(4 * MN + h * MN + mc), l);
               tmem_wait_ld();
+              if constexpr (kApart) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  v[j] = __float_as_uint(fmaf(__uint_as_float(l[j]), 1.0f / MoeHidden<T>::kScale,
+                                              __uint_as_float(v[j])));
+              }
 #pragma unroll
               for (int j = 0; j < 16; ++j) {  // (a branch a token: 64 tokens 1 us longer)
                 const float sum = fmaf(w[j], __uint_as_float(v[j]) + vb[h], y[h][mc + j]);
