@@ -125,11 +125,11 @@ __device__ __forceinline__ float gelu_erf_rel(float x) {
   q = fmaf(q, t, 0.21568267047405243f);
   q = fmaf(q, t, 0.21133993566036224f);
   const float ec = q * t * ex2_hw(-1.4426950408889634f * a * a);  // erfc(a)
-  const float h = 0.5f * x;
-  return x >= 0.0f ? fmaf(-h, ec, x) : h * ec;
+  return x * (x >= 0.0f ? fmaf(-0.5f, ec, 1.0f) : 0.5f * ec);  // (+inf stays: no x - x ec / 2)
 }
 
-// The activations to a few fp32 ulp of the value itself, tails included, for
+// The activations to a few fp32 ulp of the value itself, tails included (but what is
+// below some 2^-120 may become zero), for
 // the 8-bit and the mixture-of-experts kernels: SiLU and GELU-tanh as
 // x / (1 + exp(-z)) (0.5 (1 + tanh u) = 1 / (1 + exp(-2u)), which has no
 // cancellation where x is negative) on the hardware's ex2 and rcp.  GELU-erf is

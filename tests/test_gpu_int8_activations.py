@@ -63,3 +63,21 @@ def test_whole_range(act, dtype, kernel):
     off = (got.cpu().double() - y).abs() - tol
     i = int(off.argmax())
     assert off[i] <= 0, f"act({x[i].item()}): got {got[i].item()}, want {y[i].item()} +- {tol[i].item()}"
+
+
+@pytest.mark.parametrize("kernel", ["decode", "umma"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", list(RANGE))
+def test_infinite_and_nan_biases(act, dtype, kernel):
+    """Each in its column alone; where the definition gives NaN, NaN."""
+    inf, nan = float("inf"), float("nan")
+    b = torch.tensor([inf, -inf, nan, 1.0, torch.finfo(dtype).max, -torch.finfo(dtype).max, -1.0,
+                      0.0], dtype=dtype, device=DEV)
+    zero = torch.zeros(3, 16, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV)
+    W = torch.zeros(8, 16, dtype=torch.int8, device=DEV), torch.ones(8, device=DEV)
+    got = int8_linear(zero, W, b, act, dtype=dtype, kernel=kernel).cpu().double()
+    y = _act(b.cpu().double(), act)
+    assert torch.equal(torch.isnan(got), torch.isnan(y).expand(3, 8)), (got, y)
+    keep = ~torch.isnan(y)
+    want = y[keep].to(dtype).double().expand(3, -1)
+    assert torch.allclose(got[:, keep], want, rtol=2 * torch.finfo(dtype).eps, atol=0), (got, y)
