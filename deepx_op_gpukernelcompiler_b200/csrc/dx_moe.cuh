@@ -30,9 +30,13 @@
 //     Between the phases the CTAs wait for one another, with the first weights
 //     of phase 2 already on their way.
 //
+// The hidden rows have a place for every token of every chosen expert, so that a token
+// tile is one box; rows that nobody wrote are loaded and multiplied too (64 tokens: 16 KB
+// of token tiles, from L2, beside 32 KB of weights).
+//
 // Both launches (us, weights from HBM; the chosen experts' bytes at the measured copy
-// rate): 1 token, 2 of 8 experts of 4096 x 14336 120 (108); 8 tokens, 8 of 64 of 2048 x
-// 1024 95 (81); 64 tokens of the same 151 (123); 33 tokens, 4 of 16 of 1032 x 2824 71 (43).
+// rate): 1 token, 2 of 8 experts of 4096 x 14336 117 (108); 8 tokens, 8 of 64 of 2048 x
+// 1024 96 (81); 64 tokens of the same 145 (123); 33 tokens, 4 of 16 of 1032 x 2824 69 (43).
 //
 // Every wait is bounded, as in dx_umma_gemm.cuh.
 #pragma once

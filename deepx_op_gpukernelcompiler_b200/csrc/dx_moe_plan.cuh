@@ -94,7 +94,9 @@ __device__ __forceinline__ MoePhase moe_phase(const Params& p, int chosen, bool 
   f.whole = f.tiles / grid * grid;
   // Fewer tiles than CTAs, and short ones: joining partial sums costs more than the K
   // blocks it saves the CTAs that have a tile (20 tokens, 2 of 60 experts of 1024 x 512:
-  // 32.4 us whole, 35.1 split; 1 token, 1 of 8 of 2048 x 4096: 42.6 and 27.1).
+  // 32.4 us whole, 35.1 split; 1 token, 1 of 8 of 2048 x 4096: 42.6 and 27.1).  Phase 2's
+  // tiles are not short: each takes the K blocks of every chosen expert, and they are
+  // few (D / 256), so whole ones would leave most CTAs without work.
   if (!second && f.whole == 0 && f.per_tile - f.tiles * f.per_tile / grid <= kMoeWholeBlocks)
     f.whole = f.tiles;
   const int units = (f.tiles - f.whole) * f.per_tile;
